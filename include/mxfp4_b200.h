@@ -48,7 +48,7 @@ const char* mxb_version(void);
 /* Number of bounded pipeline waits that gave up on the current device since
  * the library was loaded (or last reset), summed over every kernel of the
  * library that waits on an mbarrier: the quantizers, the column / split FP8
- * converters and the GEMM (0 in correct operation; a non-zero value means a
+ * converters, the GEMM and the experts' products (0 in correct operation; a non-zero value means a
  * kernel abandoned its work and its outputs are invalid).  Synchronises.
  * 0xFFFFFFFF if the counters cannot be read. */
 unsigned int mxb_wait_timeouts(void);
@@ -270,6 +270,117 @@ mxb_status mxb_gemm_mxfp4(const void* a_codes, const void* a_scales_swizzled, co
                           const void* b_scales_swizzled, int64_t M, int64_t N, int64_t K, void* c,
                           mxb_stream_t stream);
 unsigned int mxb_gemm_wait_timeouts(void);
+
+/* ------------------------------------------------------------ MXFP4 experts
+ * The experts of a mixture-of-experts layer after the dispatch and the permute:
+ * rows sorted by expert, expert e owning the next m_splits[e] rows.  m_splits is
+ * an int32 DEVICE array [E], read by the kernels (no host synchronisation);
+ * negative entries count as 0, rows beyond their sum belong to nobody and their
+ * outputs are not written, and rows beyond M are never touched.  E <=
+ * MXB_MAX_EXPERTS; m_splits may be NULL for E = 1 (all M rows).  No reference
+ * counterparts (the reference hands these steps to Transformer Engine's grouped
+ * GEMM on converted FP8 operands, transformer_engine-2.8.diff). */
+#define MXB_MAX_EXPERTS 512
+
+/* Activation of an epilogue, on the f32 accumulator. */
+typedef enum {
+  MXB_ACT_NONE = 0,
+  MXB_ACT_RELU = 1,
+  MXB_ACT_RELU2 = 2,     /* max(z, 0)^2 */
+  MXB_ACT_SILU = 3,
+  MXB_ACT_GELU = 4,      /* with erf */
+  MXB_ACT_GELU_TANH = 5, /* tanh form */
+  MXB_ACT_SWIGLU = 6     /* silu(z[:, :N/2]) * z[:, N/2:]; the result has N/2 columns */
+} mxb_activation;
+
+/* What happens to z = A . B^T before it is written; a zeroed struct with c_ld =
+ * the result's width writes z as it is.  Pitches (ld) in elements, multiples of
+ * 8; pointers 16-byte aligned. */
+typedef struct {
+  const void* bias;     /* [E, N] added to z, or NULL */
+  int32_t bias_f32;     /* bias is float (else bf16) */
+  int32_t activation;   /* mxb_activation */
+  const void* residual; /* bf16 [M, W] added after the activation, or NULL (W = result width) */
+  int64_t residual_ld;
+  void* pre; /* bf16 [M, N]: z (bias included) before the activation, or NULL */
+  int64_t pre_ld;
+  int64_t c_ld;
+  void* c_codes;  /* rowwise MXFP4 of the BF16 result: codes [M, W/2] and scales [M, W/32] */
+  void* c_scales; /* (W % 32 == 0), as mxb_per_token_group_quant_fp4 writes them, or both NULL */
+} mxb_epilogue;
+
+/* Row-major E8M0 scales of E stacked weights [E, N, S] -> the 128x4-tile layout
+ * of mxb_swizzle_scales, every one of an expert's `parts` equal row ranges in
+ * tiles of its own: out [E, parts * round_up(N / parts, 128), round_up(S, 4)],
+ * zero padding.  parts = 2 for a gate / up projection (MXB_ACT_SWIGLU), else 1.
+ * Done once per weight update. */
+mxb_status mxb_swizzle_scales_grouped(const void* scales, int64_t E, int64_t N, int64_t S,
+                                      int32_t parts, void* out, mxb_stream_t stream);
+
+/* The experts' products on the tcgen05 tensor cores (kind::mxf4 block_scale,
+ * f32 accumulation): for the rows r of expert e
+ *   z[r] = A[r] . B_e^T + bias_e,  pre[r] = bf16(z[r]),
+ *   c[r] = bf16(act(z[r]) + residual[r]).
+ * a_codes [M, K/2] / a_scales [M, K/32] as the rowwise quantizer or the permute
+ * writes them, at any pitch in bytes (a_codes 16-byte aligned with a pitch of a
+ * multiple of 16; wire rows qualify); b_codes [E, N, K/2], b_scales from
+ * mxb_swizzle_scales_grouped.  K % 32 == 0, N % 8 == 0 (MXB_ACT_SWIGLU: N % 16).
+ * c bf16 [M, W], W = N (MXB_ACT_SWIGLU: N / 2), may be NULL if pre or c_codes is
+ * given.  With the transposed weights' codes (the columnwise quantize) the same
+ * call is the input gradient.  E = 1 is a dense layer. */
+mxb_status mxb_grouped_gemm_mxfp4(const void* a_codes, int64_t a_codes_pitch, const void* a_scales,
+                                  int64_t a_scales_pitch, int64_t M, const int32_t* m_splits,
+                                  int32_t E, const void* b_codes, const void* b_scales, int64_t N,
+                                  int64_t K, const mxb_epilogue* epilogue, void* c,
+                                  mxb_stream_t stream);
+
+/* The experts' weight gradients: dw[e] [N, K] = sum over the rows r of expert e
+ * of dy[r]^T x[r], with dy bf16 [M, N] (pitch dy_ld elements, a multiple of 8)
+ * and x the saved MXFP4 rows (codes [M, K/2] and E8M0 scales [M, K/32], pitches
+ * in bytes, codes 16-byte aligned).  The MXFP4 values are exact in BF16 (those
+ * of the E8M0 byte 255 are NaN; a magnitude beyond BF16's range is infinite) and
+ * multiplied on the tcgen05 tensor cores with f32 accumulation.  dw is float
+ * [E, N, K] (dw_f32) or bf16; accumulate (float only) adds to it.  An expert
+ * without rows gets zeros (or is left as it is).  N % 8 == 0, K % 32 == 0. */
+mxb_status mxb_grouped_wgrad_mxfp4(const void* dy, int64_t dy_ld, const void* x_codes,
+                                   int64_t x_codes_pitch, const void* x_scales,
+                                   int64_t x_scales_pitch, int64_t M, const int32_t* m_splits,
+                                   int32_t E, int64_t N, int64_t K, void* dw, int32_t dw_f32,
+                                   int32_t accumulate, mxb_stream_t stream);
+
+/* The gradient of the epilogue: dz = dy * act'(pre) (MXB_ACT_SWIGLU: dz[:, :N/2] =
+ * dy * up * silu'(gate), dz[:, N/2:] = dy * silu(gate)) and dbias[e] = the sum of
+ * dz over expert e's rows (f32, before dz is rounded, summed in a fixed order;
+ * zeros for an expert without rows).  dy bf16 [M, W], pre and dz bf16 [M, N], all
+ * contiguous; dz, (dz_codes, dz_scales) = the rowwise MXFP4 of dz (N % 32 == 0,
+ * MXB_ACT_SWIGLU: N % 64 == 0), and dbias float [E, N] may each be NULL.  N % 8 == 0
+ * (MXB_ACT_SWIGLU: N % 16).  pre may be NULL for MXB_ACT_NONE.  workspace: DEVICE,
+ * 16-byte aligned, mxb_bias_act_grad_workspace(M, E, N) bytes, needed only for
+ * dbias.  The residual's gradient is dy. */
+mxb_status mxb_bias_act_grad(const void* dy, const void* pre, int64_t M, const int32_t* m_splits,
+                             int32_t E, int64_t N, int32_t activation, void* dz, void* dz_codes,
+                             void* dz_scales, float* dbias, void* workspace,
+                             int64_t workspace_bytes, mxb_stream_t stream);
+int64_t mxb_bias_act_grad_workspace(int64_t M, int32_t E, int64_t N);
+
+/* The way back of mxb_moe_permute_mxfp4: out[t] = bf16(sum over k < topk, in
+ * order, with 0 <= map[t * map_pitch + k] < R of weight[t * topk + k] *
+ * y[map[t * map_pitch + k]]), y bf16 [R, H], out bf16 [T, H], weight float DEVICE
+ * [T, topk] or NULL (all ones).  A token without rows gets zeros.  map int32
+ * DEVICE; mxb_moe_make_row_id_map's map is map_pitch = 2E + 1, topk = E.  H % 8 ==
+ * 0, 1 <= topk <= 1024. */
+mxb_status mxb_moe_unpermute(const void* y, int64_t R, int64_t H, const int32_t* map,
+                             int64_t map_pitch, int32_t topk, const float* weight, int64_t T,
+                             void* out, mxb_stream_t stream);
+/* Its gradient: dy[map[t, k]] = bf16(weight[t, k] * dout[t]) and dweight[t, k] =
+ * <dout[t], y[map[t, k]]> in f32 (0 where there is no row).  Each row of y is
+ * named at most once (dy of rows that are not named is left as it is).  dy bf16 [R, H],
+ * (dy_codes, dy_scales) = the rowwise MXFP4 of dy (H % 32 == 0), and dweight float
+ * [T, topk] may each be NULL; y is needed for dweight only. */
+mxb_status mxb_moe_unpermute_grad(const void* dout, const void* y, int64_t R, int64_t H,
+                                  const int32_t* map, int64_t map_pitch, int32_t topk,
+                                  const float* weight, int64_t T, void* dy, void* dy_codes,
+                                  void* dy_scales, float* dweight, mxb_stream_t stream);
 
 /* ------------------------------------------------------------ per-token FP8 */
 

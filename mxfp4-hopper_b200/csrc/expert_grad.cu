@@ -1,0 +1,422 @@
+// The streaming operators around the experts' products (sm_100a):
+//   * bias_act_grad: dz = dy * act'(pre), the rowwise MXFP4 of dz for the input
+//     gradient's product, and the bias gradient, in one pass over dy and pre;
+//   * moe_unpermute: the weighted sum of each token's expert rows;
+//   * moe_unpermute_grad: its gradient towards the rows and the weights.
+// All are bound by HBM: every operand is read once in 16-byte pieces, with
+// several rows' loads in flight per thread.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+
+#include "capi_util.h"
+#include "common.cuh"
+#include "epilogue.cuh"
+#include "groups.cuh"
+
+namespace mxb {
+namespace {
+
+// ---------------------------------------------------------------- bias_act_grad
+// A CTA takes kGradRows rows of one expert by 256 columns of dy: a warp a row, a
+// lane eight columns, four rows in flight.  Column sums stay in registers over a
+// warp's rows, meet in shared memory in warp order, and leave as one partial sum
+// per CTA; a second kernel adds an expert's partials in row order, so the bias
+// gradient does not depend on scheduling.  With at most kGradRows rows there is
+// one CTA per expert and column range, which writes dbias itself.
+constexpr int kGradRows = 128;
+constexpr int kGradThreads = 256, kGradWarps = 8, kGradCols = 256;
+
+__device__ __forceinline__ int grad_chunks(int rows) {
+  return rows > kGradRows ? (rows + kGradRows - 1) / kGradRows : 1;
+}
+int64_t most_grad_chunks(int64_t M, int64_t E) { return M / kGradRows + E; }
+
+struct ActGradArgs {
+  const uint8_t *dy, *pre;
+  const int32_t* m_splits;
+  int64_t M;
+  int E, N, width;
+  uint8_t *dz, *codes, *scales;
+  float* sums;  // [chunks, N] partials, or dbias itself; NULL: no bias gradient
+};
+
+template <int kAct>
+__global__ void __launch_bounds__(kGradThreads) act_grad_kernel(const ActGradArgs p, int slabs) {
+  constexpr bool kGlu = kAct == MXB_ACT_SWIGLU;
+  constexpr int kParts = kGlu ? 2 : 1;
+  __shared__ int32_t table[kGroupTableInts];
+  __shared__ float red[kParts][kGradWarps][kGradCols];
+  const GroupTable g{table, table + p.E + 1};
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  if (warp == 0) build_groups(g, p.m_splits, p.E, p.M, grad_chunks);
+  __syncthreads();
+  const int chunk = (int)(blockIdx.x / slabs), slab = (int)(blockIdx.x % slabs);
+  if (chunk >= g.tile[p.E]) return;
+  const int e = find_group(g.tile, p.E, chunk);
+  const int r0 = g.off[e] + (chunk - g.tile[e]) * kGradRows;
+  const int r1 = min(r0 + kGradRows, g.off[e + 1]);
+  const int n = slab * kGradCols + lane * 8;
+  const bool in = n < p.width;
+  float sum[kParts][8] = {};
+  constexpr int kRows = 4;
+  for (int r = r0 + warp; r < r1; r += kGradWarps * kRows) {
+    uint4 d[kRows], z[kParts][kRows];
+#pragma unroll
+    for (int q = 0; q < kRows; ++q) {
+      const int64_t row = r + q * kGradWarps;
+      if (in && row < r1) {
+        d[q] = ld_stream_v4(p.dy + (row * p.width + n) * 2);
+        if (kAct != MXB_ACT_NONE) {
+#pragma unroll
+          for (int h = 0; h < kParts; ++h)
+            z[h][q] = ld_stream_v4(p.pre + (row * p.N + h * p.width + n) * 2);
+        }
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < kRows; ++q) {
+      const int64_t row = r + q * kGradWarps;
+      if (row >= r1) break;  // the same for the whole warp
+      float dv[8], o[kParts][8];
+      if (in) {
+        unpack8_bf16(d[q], dv);
+        if constexpr (kGlu) {
+          float a[8], b[8];
+          unpack8_bf16(z[0][q], a);
+          unpack8_bf16(z[1][q], b);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float s = logistic(a[k]);
+            o[0][k] = dv[k] * b[k] * s * (1.0f + a[k] * (1.0f - s));
+            o[1][k] = dv[k] * a[k] * s;
+          }
+        } else {
+          float a[8] = {};
+          if (kAct != MXB_ACT_NONE) unpack8_bf16(z[0][q], a);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) o[0][k] = dv[k] * act_slope<kAct>(a[k]);
+        }
+#pragma unroll
+        for (int h = 0; h < kParts; ++h) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) sum[h][k] += o[h][k];
+          if (p.dz)
+            *reinterpret_cast<uint4*>(p.dz + (row * p.N + h * p.width + n) * 2) = pack8_bf16(o[h]);
+        }
+      }
+      if (p.codes) {
+#pragma unroll
+        for (int h = 0; h < kParts; ++h)
+          quant_quad(p.codes, p.scales, o[h], in, row * p.N + h * p.width + n);
+      }
+    }
+  }
+  if (!p.sums) return;
+#pragma unroll
+  for (int h = 0; h < kParts; ++h)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) red[h][warp][lane * 8 + k] = sum[h][k];
+  __syncthreads();
+  const int col = slab * kGradCols + t;
+  if (col < p.width) {
+#pragma unroll
+    for (int h = 0; h < kParts; ++h) {
+      float s = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kGradWarps; ++w) s += red[h][w][t];
+      p.sums[(int64_t)chunk * p.N + h * p.width + col] = s;
+    }
+  }
+}
+
+// dbias[e][n] = the sum of expert e's partials: 32 columns a CTA, eight warps
+// taking every eighth partial, added in warp order.
+__global__ void __launch_bounds__(kGradThreads) bias_sum_kernel(const float* __restrict__ partial,
+                                                                const int32_t* m_splits, int64_t M,
+                                                                int E, int N,
+                                                                float* __restrict__ dbias) {
+  __shared__ int32_t table[kGroupTableInts];
+  __shared__ float red[kGradWarps][32];
+  const GroupTable g{table, table + E + 1};
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 0) build_groups(g, m_splits, E, M, grad_chunks);
+  __syncthreads();
+  const int e = blockIdx.y, n = blockIdx.x * 32 + lane;
+  float s = 0.0f;
+  if (n < N) {
+    const int end = g.tile[e + 1];
+#pragma unroll 4
+    for (int c = g.tile[e] + warp; c < end; c += kGradWarps) s += partial[(int64_t)c * N + n];
+  }
+  red[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && n < N) {
+    float total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kGradWarps; ++w) total += red[w][lane];
+    dbias[(int64_t)e * N + n] = total;
+  }
+}
+
+template <int kAct>
+void launch_act_grad(const ActGradArgs& p, int64_t blocks, int slabs, cudaStream_t s) {
+  act_grad_kernel<kAct><<<(unsigned)blocks, kGradThreads, 0, s>>>(p, slabs);
+}
+
+// ---------------------------------------------------------------- unpermute
+// A thread owns eight columns of a token and has its rows' loads, eight at a
+// time, in flight together; the sum runs over k in order, in f32.
+constexpr int kUnpThreads = 256;
+constexpr int kUnpBatch = 8;
+
+struct UnpermuteMap {
+  const int32_t* map;
+  int64_t pitch;
+  const float* weight;
+  int topk;
+  int64_t R;
+  // row of (t, k), or -1
+  __device__ __forceinline__ int64_t row(int64_t t, int k) const {
+    const int32_t r = map[t * pitch + k];
+    return r >= 0 && r < R ? r : -1;
+  }
+  __device__ __forceinline__ float w(int64_t t, int k) const {
+    return weight ? weight[t * topk + k] : 1.0f;
+  }
+};
+
+__global__ void __launch_bounds__(kUnpThreads) unpermute_kernel(const uint8_t* __restrict__ y,
+                                                                const UnpermuteMap m, int64_t T,
+                                                                int64_t H,
+                                                                uint8_t* __restrict__ out) {
+  const int64_t per_row = H / 8, items = T * per_row;
+  for (int64_t i = (int64_t)blockIdx.x * kUnpThreads + threadIdx.x; i < items;
+       i += (int64_t)gridDim.x * kUnpThreads) {
+    const int64_t t = i / per_row, c = i % per_row;
+    float acc[8] = {};
+    for (int k0 = 0; k0 < m.topk; k0 += kUnpBatch) {
+      uint4 v[kUnpBatch];
+      float w[kUnpBatch];
+      bool there[kUnpBatch];
+#pragma unroll
+      for (int k = 0; k < kUnpBatch; ++k) {
+        const int64_t r = k0 + k < m.topk ? m.row(t, k0 + k) : -1;
+        there[k] = r >= 0;
+        if (there[k]) {
+          v[k] = ld_stream_v4(y + (r * H + c * 8) * 2);
+          w[k] = m.w(t, k0 + k);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kUnpBatch; ++k) {
+        if (!there[k]) continue;
+        float x[8];
+        unpack8_bf16(v[k], x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] += w[k] * x[j];
+      }
+    }
+    *reinterpret_cast<uint4*>(out + (t * H + c * 8) * 2) = pack8_bf16(acc);
+  }
+}
+
+// One CTA per token: dout's chunk is read once per eight rows, each row's dot
+// product is summed over lanes and warps in a fixed order.
+__global__ void __launch_bounds__(kUnpThreads) unpermute_grad_kernel(
+    const uint8_t* __restrict__ dout, const uint8_t* __restrict__ y, const UnpermuteMap m,
+    int64_t T, int64_t H, uint8_t* __restrict__ dy, uint8_t* __restrict__ codes,
+    uint8_t* __restrict__ scales, float* __restrict__ dweight) {
+  __shared__ float red[kUnpThreads / 32][kUnpBatch];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t per_row = H / 8;
+  for (int64_t t = blockIdx.x; t < T; t += gridDim.x) {
+    for (int k0 = 0; k0 < m.topk; k0 += kUnpBatch) {
+      int64_t row[kUnpBatch];
+      float w[kUnpBatch], dot[kUnpBatch] = {};
+#pragma unroll
+      for (int k = 0; k < kUnpBatch; ++k) {
+        row[k] = k0 + k < m.topk ? m.row(t, k0 + k) : -1;
+        w[k] = row[k] >= 0 ? m.w(t, k0 + k) : 0.0f;
+      }
+      for (int64_t c0 = warp * 32; c0 < per_row; c0 += kUnpThreads) {  // the same for a warp
+        const int64_t c = c0 + lane;
+        const bool in = c < per_row;
+        uint4 d = make_uint4(0u, 0u, 0u, 0u), v[kUnpBatch];
+        if (in) d = *reinterpret_cast<const uint4*>(dout + (t * H + c * 8) * 2);
+        if (dweight) {
+#pragma unroll
+          for (int k = 0; k < kUnpBatch; ++k)
+            if (in && row[k] >= 0) v[k] = ld_stream_v4(y + (row[k] * H + c * 8) * 2);
+        }
+        float dv[8];
+        unpack8_bf16(d, dv);
+#pragma unroll
+        for (int k = 0; k < kUnpBatch; ++k) {
+          if (row[k] < 0) continue;  // the same for the whole CTA
+          if (dweight && in) {
+            float x[8];
+            unpack8_bf16(v[k], x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) dot[k] += dv[j] * x[j];
+          }
+          if (dy || codes) {
+            float o[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] = w[k] * dv[j];
+            if (dy && in)
+              *reinterpret_cast<uint4*>(dy + (row[k] * H + c * 8) * 2) = pack8_bf16(o);
+            if (codes) quant_quad(codes, scales, o, in, row[k] * H + c * 8);
+          }
+        }
+      }
+      if (!dweight) continue;
+#pragma unroll
+      for (int k = 0; k < kUnpBatch; ++k) {
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) dot[k] += __shfl_xor_sync(0xffffffffu, dot[k], d);
+        if (lane == 0) red[warp][k] = dot[k];
+      }
+      __syncthreads();
+      if (threadIdx.x < kUnpBatch && k0 + (int)threadIdx.x < m.topk) {
+        float s = 0.0f;
+#pragma unroll
+        for (int q = 0; q < kUnpThreads / 32; ++q) s += red[q][threadIdx.x];
+        dweight[t * m.topk + k0 + threadIdx.x] = s;
+      }
+      __syncthreads();
+    }
+  }
+}
+
+mxb_status check_unpermute(const char* what, int64_t R, int64_t H, int64_t map_pitch, int32_t topk,
+                           int64_t T) {
+  MXB_REQUIRE(T >= 0 && R >= 0 && R <= INT32_MAX && H >= 0 && H % 8 == 0, MXB_ERR_INVALID_ARGUMENT,
+              "%s: need T >= 0, 0 <= R < 2^31 and H %% 8 == 0 (T=%lld R=%lld H=%lld)", what,
+              (long long)T, (long long)R, (long long)H);
+  MXB_REQUIRE(topk >= 1 && topk <= 1024 && map_pitch >= topk, MXB_ERR_INVALID_ARGUMENT,
+              "%s: need 1 <= topk <= 1024 and map_pitch >= topk (topk=%d map_pitch=%lld)", what,
+              topk, (long long)map_pitch);
+  return MXB_OK;
+}
+
+}  // namespace
+}  // namespace mxb
+
+using namespace mxb;
+
+extern "C" int64_t mxb_bias_act_grad_workspace(int64_t M, int32_t E, int64_t N) {
+  if (M <= kGradRows || E < 1 || N < 1) return 0;
+  return most_grad_chunks(M, E) * N * 4;
+}
+
+extern "C" mxb_status mxb_bias_act_grad(const void* dy, const void* pre, int64_t M,
+                                        const int32_t* m_splits, int32_t E, int64_t N,
+                                        int32_t activation, void* dz, void* dz_codes,
+                                        void* dz_scales, float* dbias, void* workspace,
+                                        int64_t workspace_bytes, mxb_stream_t stream) {
+  const char* const what = "bias_act_grad";
+  MXB_REQUIRE(activation >= MXB_ACT_NONE && activation <= MXB_ACT_SWIGLU, MXB_ERR_INVALID_ARGUMENT,
+              "%s: unknown activation %d", what, activation);
+  const int parts = activation == MXB_ACT_SWIGLU ? 2 : 1;
+  MXB_REQUIRE(M >= 0 && M <= INT32_MAX && E >= 1 && E <= MXB_MAX_EXPERTS, MXB_ERR_INVALID_ARGUMENT,
+              "%s: need 0 <= M < 2^31 and 1 <= E <= %d (M=%lld E=%d)", what, MXB_MAX_EXPERTS,
+              (long long)M, E);
+  MXB_REQUIRE(N >= 0 && N <= INT32_MAX - 512 && N % (8 * parts) == 0, MXB_ERR_INVALID_ARGUMENT,
+              "%s: need N %% %d == 0 (N=%lld)", what, 8 * parts, (long long)N);
+  MXB_REQUIRE(!dz_codes == !dz_scales && (!dz_codes || N % (32 * parts) == 0),
+              MXB_ERR_INVALID_ARGUMENT,
+              "%s: a quantized dz needs both dz_codes and dz_scales and N %% %d == 0", what,
+              32 * parts);
+  if (N == 0) return MXB_OK;
+  MXB_REQUIRE(m_splits || E == 1, MXB_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  MXB_REQUIRE(dz || dz_codes || dbias, MXB_ERR_INVALID_ARGUMENT, "%s: no output", what);
+  const cudaStream_t s = to_cuda(stream);
+  if (M == 0) {
+    if (dbias && cudaMemsetAsync(dbias, 0, (size_t)E * N * 4, s) != cudaSuccess)
+      return launch_status(what);
+    return MXB_OK;
+  }
+  MXB_REQUIRE(dy && (pre || activation == MXB_ACT_NONE), MXB_ERR_INVALID_ARGUMENT,
+              "%s: null pointer", what);
+  MXB_REQUIRE(aligned(dy, 16) && aligned(pre, 16) && aligned(dz, 16) && aligned(dz_codes, 16) &&
+                  aligned(dbias, 4) && aligned(workspace, 16),
+              MXB_ERR_MISALIGNED, "%s: operands must be 16-byte aligned", what);
+  const int64_t need = dbias ? mxb_bias_act_grad_workspace(M, E, N) : 0;
+  MXB_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), MXB_ERR_INVALID_ARGUMENT,
+              "%s: workspace of %lld bytes needed, %lld given", what, (long long)need,
+              (long long)workspace_bytes);
+  ActGradArgs p;
+  p.dy = (const uint8_t*)dy;
+  p.pre = (const uint8_t*)pre;
+  p.m_splits = m_splits;
+  p.M = M;
+  p.E = E;
+  p.N = (int)N;
+  p.width = (int)(N / parts);
+  p.dz = (uint8_t*)dz;
+  p.codes = (uint8_t*)dz_codes;
+  p.scales = (uint8_t*)dz_scales;
+  p.sums = !dbias ? nullptr : need ? (float*)workspace : dbias;
+  const int slabs = (int)cdiv(p.width, kGradCols);
+  const int64_t blocks = (M <= kGradRows ? (int64_t)E : most_grad_chunks(M, E)) * slabs;
+  MXB_REQUIRE(blocks <= INT32_MAX, MXB_ERR_INVALID_ARGUMENT, "%s: too many blocks", what);
+  switch (activation) {
+    case MXB_ACT_NONE: launch_act_grad<MXB_ACT_NONE>(p, blocks, slabs, s); break;
+    case MXB_ACT_RELU: launch_act_grad<MXB_ACT_RELU>(p, blocks, slabs, s); break;
+    case MXB_ACT_RELU2: launch_act_grad<MXB_ACT_RELU2>(p, blocks, slabs, s); break;
+    case MXB_ACT_SILU: launch_act_grad<MXB_ACT_SILU>(p, blocks, slabs, s); break;
+    case MXB_ACT_GELU: launch_act_grad<MXB_ACT_GELU>(p, blocks, slabs, s); break;
+    case MXB_ACT_GELU_TANH: launch_act_grad<MXB_ACT_GELU_TANH>(p, blocks, slabs, s); break;
+    default: launch_act_grad<MXB_ACT_SWIGLU>(p, blocks, slabs, s); break;
+  }
+  if (need) {
+    const mxb_status st = launch_status(what);
+    if (st != MXB_OK) return st;
+    bias_sum_kernel<<<dim3((unsigned)cdiv(N, 32), (unsigned)E), kGradThreads, 0, s>>>(
+        (const float*)workspace, m_splits, M, E, (int)N, dbias);
+  }
+  return launch_status(what);
+}
+
+extern "C" mxb_status mxb_moe_unpermute(const void* y, int64_t R, int64_t H, const int32_t* map,
+                                        int64_t map_pitch, int32_t topk, const float* weight,
+                                        int64_t T, void* out, mxb_stream_t stream) {
+  const char* const what = "moe_unpermute";
+  const mxb_status st = check_unpermute(what, R, H, map_pitch, topk, T);
+  if (st != MXB_OK) return st;
+  if (T == 0 || H == 0) return MXB_OK;
+  MXB_REQUIRE((y || R == 0) && map && out, MXB_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  MXB_REQUIRE(aligned(y, 16) && aligned(out, 16) && aligned(map, 4) && aligned(weight, 4),
+              MXB_ERR_MISALIGNED, "%s: y and out must be 16-byte aligned", what);
+  const UnpermuteMap m{map, map_pitch, weight, topk, R};
+  const int64_t blocks = std::min<int64_t>(cdiv(T * (H / 8), kUnpThreads), INT32_MAX);
+  unpermute_kernel<<<(unsigned)blocks, kUnpThreads, 0, to_cuda(stream)>>>((const uint8_t*)y, m, T,
+                                                                          H, (uint8_t*)out);
+  return launch_status(what);
+}
+
+extern "C" mxb_status mxb_moe_unpermute_grad(const void* dout, const void* y, int64_t R, int64_t H,
+                                             const int32_t* map, int64_t map_pitch, int32_t topk,
+                                             const float* weight, int64_t T, void* dy,
+                                             void* dy_codes, void* dy_scales, float* dweight,
+                                             mxb_stream_t stream) {
+  const char* const what = "moe_unpermute_grad";
+  const mxb_status st = check_unpermute(what, R, H, map_pitch, topk, T);
+  if (st != MXB_OK) return st;
+  MXB_REQUIRE(!dy_codes == !dy_scales && (!dy_codes || H % 32 == 0), MXB_ERR_INVALID_ARGUMENT,
+              "%s: a quantized dy needs both dy_codes and dy_scales and H %% 32 == 0", what);
+  MXB_REQUIRE(dy || dy_codes || dweight, MXB_ERR_INVALID_ARGUMENT, "%s: no output", what);
+  if (T == 0) return MXB_OK;
+  MXB_REQUIRE((dout || H == 0) && map && (y || !dweight || R == 0 || H == 0),
+              MXB_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  MXB_REQUIRE(aligned(dout, 16) && aligned(y, 16) && aligned(dy, 16) && aligned(dy_codes, 16) &&
+                  aligned(map, 4) && aligned(weight, 4) && aligned(dweight, 4),
+              MXB_ERR_MISALIGNED, "%s: operands must be 16-byte aligned", what);
+  const UnpermuteMap m{map, map_pitch, weight, topk, R};
+  unpermute_grad_kernel<<<(unsigned)std::min<int64_t>(T, INT32_MAX), kUnpThreads, 0,
+                          to_cuda(stream)>>>(
+      (const uint8_t*)dout, (const uint8_t*)y, m, T, H, (uint8_t*)dy, (uint8_t*)dy_codes,
+      (uint8_t*)dy_scales, dweight);
+  return launch_status(what);
+}

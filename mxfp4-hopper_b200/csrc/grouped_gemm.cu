@@ -1,0 +1,1019 @@
+// The experts' MXFP4 products with a fused epilogue (sm_100a): for the rows r of
+// expert e, z[r] = A[r] . B_e^T + bias_e, c[r] = act(z[r]) + residual[r].
+//
+// Rows are sorted by expert and the split is ragged and only known on the
+// device: every CTA builds the running sums of m_splits in shared memory and
+// walks tiles of (expert, row block, column block).  A's rows start anywhere, so
+// its E8M0 bytes are read row by row from the row-major layout that the
+// quantizer and the permute write, and put into the 128x4 atoms of the tcgen05
+// block-scale layout on the way to shared memory; a tile's rows past its
+// group's end are computed and not written.
+//
+// Two kernels, chosen by grouped_plan() below:
+//   wide    128 rows x 256 weight rows a tile: the rows are the MMA's M side.
+//   narrow  16 or 64 rows x 128 (gated: 256) weight rows a tile: the weights are
+//           the M side, so that a few rows do not pay for 128.  A cluster of up
+//           to 8 CTAs splits K; the partial accumulators meet in distributed
+//           shared memory, always summed in the same order.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+
+#include "capi_util.h"
+#include "common.cuh"
+#include "epilogue.cuh"
+#include "groups.cuh"
+#include "host_util.h"
+#include "qrow.cuh"
+#include "tma.cuh"
+#include "umma.cuh"
+
+namespace mxb {
+namespace {
+
+constexpr int kStepK = 256;  // elements of K per pipeline stage: 128 code bytes, 8 scales a row
+
+struct GroupedArgs {
+  const uint8_t* a_scales;
+  int64_t a_spitch;
+  const uint8_t* b_scales;
+  const int32_t* m_splits;
+  int64_t M;
+  int E, width, K;  // width: columns of the result (N, gated N / 2)
+  int act, bias_f32;
+  const void* bias;
+  const uint8_t* residual;
+  int64_t residual_ld;
+  uint8_t *pre, *c;
+  int64_t pre_ld, c_ld;
+  uint8_t *c_codes, *c_scales;
+};
+
+// The 8 scale bytes of one row's K step as two words (the two atoms of the
+// step); bytes past the row's K / 32 scales are zero.
+__device__ __forceinline__ uint2 row_scales(const uint8_t* row, int S, int ks, int mode) {
+  const int b0 = ks * 8;
+  uint2 w = make_uint2(0u, 0u);
+  if (mode == 8) return *reinterpret_cast<const uint2*>(row + b0);  // S % 8 == 0
+  if (mode == 4) {                                                   // S % 4 == 0
+    w.x = *reinterpret_cast<const uint32_t*>(row + b0);
+    if (b0 + 4 < S) w.y = *reinterpret_cast<const uint32_t*>(row + b0 + 4);
+    return w;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (b0 + i < S) w.x |= (uint32_t)row[b0 + i] << (8 * i);
+    if (b0 + 4 + i < S) w.y |= (uint32_t)row[b0 + 4 + i] << (8 * i);
+  }
+  return w;
+}
+__device__ __forceinline__ int scale_mode(const GroupedArgs& p) {
+  const uintptr_t any = reinterpret_cast<uintptr_t>(p.a_scales) | (uintptr_t)p.a_spitch |
+                        (uintptr_t)(p.K / 32);
+  return (any & 7) == 0 ? 8 : (any & 3) == 0 ? 4 : 1;
+}
+
+__device__ __forceinline__ float load_bias(const GroupedArgs& p, int64_t i) {
+  return p.bias_f32 ? static_cast<const float*>(p.bias)[i]
+                    : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[i]);
+}
+
+// ---------------------------------------------------------------- wide
+// One persistent CTA per SM; a tile has 128 rows and two 128-row weight boxes:
+// columns n0 .. n0 + 255 of the result, or (gated) gate and up rows of columns
+// n0 .. n0 + 127.
+//   warp 0       TMA of A's and B's codes and bulk copies of B's scale atoms
+//   warp 1       MMA issue (scale atoms to tensor memory, 4 MMAs of K = 64)
+//   warps 2-9    epilogue: two groups of four warps, each with half the columns
+//   warps 10-13  A's scale bytes: one row a thread, the next four steps' bytes
+//                in registers before they are needed
+constexpr int kWideThreads = 448;
+constexpr int kWideStages = 3;
+constexpr uint32_t kBoxBytes = 128 * 128;  // 128 rows of 128 code bytes
+constexpr uint32_t kAtoms = 2 * 512;       // scale atoms of 128 rows and one K step
+constexpr uint32_t kWideStage = 3 * kBoxBytes + 3 * kAtoms;
+constexpr uint32_t kOutBox = 128 * 64;     // 128 rows x 32 bf16 columns, 64-byte swizzle
+constexpr int kOutSlots = 4;               // per epilogue group
+constexpr uint32_t kScaleCol = 256;        // tensor memory: accumulator, then scales
+constexpr uint32_t kTmemCols = 512;
+constexpr size_t kWideSmem = 1024 + kWideStages * kWideStage + 2 * kOutSlots * kOutBox + 256 * 4 +
+                             kGroupTableInts * 4 + 128;
+static_assert(kWideSmem <= 227 * 1024, "one CTA per SM");
+
+template <bool kGlu>
+__global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
+    const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+    const __grid_constant__ CUtensorMap map_c, const __grid_constant__ CUtensorMap map_pre,
+    const __grid_constant__ CUtensorMap map_pre_up, const __grid_constant__ GroupedArgs p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  uint8_t* out_boxes = smem + kWideStages * kWideStage;
+  float* bias_s = reinterpret_cast<float*>(out_boxes + 2 * kOutSlots * kOutBox);
+  uint64_t* full = reinterpret_cast<uint64_t*>(bias_s + 256);
+  uint64_t* empty = full + kWideStages;
+  uint64_t* acc_full = empty + kWideStages;
+  uint64_t* acc_empty = acc_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 1);
+  int* failed = reinterpret_cast<int*>(tmem_slot + 1);
+  GroupTable g;
+  g.off = failed + 1;
+  g.tile = g.off + p.E + 1;
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  constexpr int kTileN = kGlu ? 128 : 256;
+  const int ntn = (p.width + kTileN - 1) / kTileN;
+  const int ksteps = (p.K + kStepK - 1) / kStepK;
+  const int S = p.K / 32, S4 = (S + 3) / 4;
+
+  if (warp == 0) {
+    build_groups(g, p.m_splits, p.E, p.M, [&](int rows) { return (rows + 127) / 128 * ntn; });
+  } else if (warp == 1) {
+    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_relinquish();
+  } else if (t == 64) {
+    for (int s = 0; s < kWideStages; ++s) {
+      mbar_init(&full[s], 1 + 4);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_init(acc_empty, 8);
+    fence_mbar_init();
+    *failed = 0;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int tiles = g.tile[p.E];
+  const int my_tiles =
+      (int)blockIdx.x < tiles ? (tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+
+  struct Tile {
+    int e, m0, n0;
+  };
+  auto tile_at = [&](int i) {
+    const int id = (int)blockIdx.x + i * (int)gridDim.x;
+    Tile r;
+    r.e = find_group(g.tile, p.E, id);
+    const int local = id - g.tile[r.e];
+    r.m0 = g.off[r.e] + local / ntn * 128;
+    r.n0 = local % ntn * kTileN;
+    return r;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------ TMA producer
+    if (lane == 0) {
+      const int nbp = (p.width + 127) / 128;  // 128-row scale blocks of a weight part
+      int issued = 0;
+      bool ok = true;
+      for (int i = 0; ok && i < my_tiles; ++i) {
+        const Tile tl = tile_at(i);
+        int row0, row1, sb0, sb1;
+        bool second = true;
+        if (kGlu) {
+          row0 = 2 * tl.e * p.width + tl.n0;
+          row1 = row0 + p.width;
+          sb0 = 2 * tl.e * nbp + tl.n0 / 128;
+          sb1 = sb0 + nbp;
+        } else {
+          row0 = tl.e * p.width + tl.n0;
+          row1 = row0 + 128;
+          sb0 = tl.e * nbp + tl.n0 / 128;
+          sb1 = sb0 + 1;
+          second = tl.n0 + 128 < p.width;  // else: stale codes, columns that are not written
+        }
+        for (int ks = 0; ks < ksteps; ++ks) {
+          const int gs = issued, s = gs % kWideStages;
+          if (gs >= kWideStages &&
+              !mbar_wait(&empty[s], (uint32_t)((gs / kWideStages - 1) & 1))) {
+            atomicExch(failed, 1);
+            ok = false;
+            break;
+          }
+          uint8_t* st = smem + s * kWideStage;
+          uint8_t* sf = st + 3 * kBoxBytes + kAtoms;
+          const uint32_t atoms = (uint32_t)min(2, S4 - 2 * ks) * 512;
+          mbar_arrive_expect_tx(&full[s],
+                                kBoxBytes + (kBoxBytes + atoms) * (second ? 2u : 1u));
+          const int kx = ks * (kStepK / 2);
+          tma_load_2d(st, &map_a, kx, tl.m0, &full[s]);
+          tma_load_2d(st + kBoxBytes, &map_b, kx, row0, &full[s]);
+          bulk_load_1d(sf, p.b_scales + ((int64_t)sb0 * S4 + 2 * ks) * 512, atoms, &full[s]);
+          if (second) {
+            tma_load_2d(st + 2 * kBoxBytes, &map_b, kx, row1, &full[s]);
+            bulk_load_1d(sf + kAtoms, p.b_scales + ((int64_t)sb1 * S4 + 2 * ks) * 512, atoms,
+                         &full[s]);
+          }
+          issued = gs + 1;
+        }
+      }
+      // do not leave while copies of this CTA are still landing
+      for (int gs = issued > kWideStages ? issued - kWideStages : 0; gs < issued; ++gs)
+        mbar_wait(&full[gs % kWideStages], (uint32_t)((gs / kWideStages) & 1));
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      bool ok = true;
+      int gs = 0;
+      for (int i = 0; ok && i < my_tiles; ++i) {
+        if (i > 0 && !mbar_wait(acc_empty, (uint32_t)((i - 1) & 1))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        for (int ks = 0; ks < ksteps; ++ks, ++gs) {
+          const int s = gs % kWideStages;
+          if (!mbar_wait(&full[s], (uint32_t)((gs / kWideStages) & 1))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint8_t* st = smem + s * kWideStage;
+          const uint8_t* sf = st + 3 * kBoxBytes;
+          const uint32_t sfc = tmem + kScaleCol + (uint32_t)(s * 24);
+          const int left = p.K - ks * kStepK;  // elements of K from this step on
+#pragma unroll
+          for (int a = 0; a < 2; ++a) {
+            if (128 * a >= left) break;
+            tc_copy_sf(sfc + 4 * a, smem_desc_sf(sf + a * 512));
+            tc_copy_sf(sfc + 8 + 8 * a, smem_desc_sf(sf + kAtoms + a * 512));
+            tc_copy_sf(sfc + 12 + 8 * a, smem_desc_sf(sf + 2 * kAtoms + a * 512));
+          }
+          const uint64_t da = smem_desc_sw128(st);
+          const uint64_t db = smem_desc_sw128(st + kBoxBytes);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (64 * j >= left) break;
+            const uint32_t sf_id = (uint32_t)(j & 1) * 2u;
+            tc_mma(tmem, da + (uint64_t)(2 * j), db + (uint64_t)(2 * j), mxf4_idesc(256, sf_id),
+                   (sfc + 4 * (j >> 1)) | (sf_id << 30), (sfc + 8 + 8 * (j >> 1)) | (sf_id << 30),
+                   (ks > 0 || j > 0) ? 1u : 0u);
+          }
+          tc_commit(&empty[s]);
+        }
+        tc_commit(acc_full);
+      }
+      if (!ok) atomicExch(failed, 1);
+    }
+  } else if (warp < 10) {
+    // ------------------------------------------------ epilogue
+    const int half = (warp - 2) >> 2, quad = warp & 3;
+    const int r = quad * 32 + lane, ht = (t - 64) & 127;
+    const bool issuer = ht == 0;
+    uint8_t* boxes = out_boxes + half * kOutSlots * kOutBox;
+    float* bias_h = bias_s + half * 128;
+    constexpr int kHalfN = kTileN / 2;  // result columns of this group
+    const int n_pre = p.pre ? (kGlu ? 2 : 1) : 0;
+    const int n_box = n_pre + (p.c ? 1 : 0);
+    const int sets = n_box == 3 ? 1 : n_box == 2 ? 2 : 4;
+    int set = 0;
+    for (int i = 0; i < my_tiles; ++i) {
+      const Tile tl = tile_at(i);
+      const int rows = min(128, g.off[tl.e + 1] - tl.m0);
+      const int nh = tl.n0 + half * kHalfN;  // first result column of this group
+      if (p.bias) {
+        // this group's 128 accumulator columns: 128 of z, or 64 gate and 64 up
+        const int col = kGlu ? nh + (ht & 63) : nh + ht;
+        const int64_t at = kGlu ? (int64_t)tl.e * 2 * p.width + (ht < 64 ? 0 : p.width) + col
+                                : (int64_t)tl.e * p.width + col;
+        bias_h[ht] = col < p.width ? load_bias(p, at) : 0.0f;
+      } else {
+        bias_h[ht] = 0.0f;
+      }
+      const bool ok = mbar_wait(acc_full, (uint32_t)(i & 1));
+      tc_fence_after();
+      const bool live = ok && !*((volatile int*)failed);
+      if (named_sync_or(1 + half, 128, !live)) break;  // the four warps leave together
+      const bool whole = rows == 128;
+      const int64_t row = (int64_t)tl.m0 + r;
+#pragma unroll 1
+      for (int ch = 0; ch < kHalfN / 32; ++ch) {
+        const int n = nh + 32 * ch;
+        if (n >= p.width) break;
+        const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
+        uint32_t acc[32];
+        float v[32], u[kGlu ? 32 : 1];
+        __syncwarp();
+        tmem_ld32(lane_base + (uint32_t)(half * kHalfN + 32 * ch), acc);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(acc[j]) + bias_h[32 * ch + j];
+        if constexpr (kGlu) {
+          tmem_ld32(lane_base + (uint32_t)(128 + half * kHalfN + 32 * ch), acc);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) u[j] = __uint_as_float(acc[j]) + bias_h[64 + 32 * ch + j];
+        }
+        // the boxes of this set have been read by the stores issued `sets` chunks ago
+        if (issuer) {
+          if (sets == 1) bulk_wait_read_all();
+          else if (sets == 2) bulk_wait_read_1();
+          else bulk_wait_read_3();
+        }
+        named_sync(1 + half, 128);
+        uint8_t* bx = boxes + set * n_box * kOutBox;
+        auto put = [&](uint8_t* box, const float* x) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            *reinterpret_cast<uint4*>(box + r * 64 + ((k ^ ((r >> 1) & 3)) << 4)) =
+                pack8_bf16(x + 8 * k);
+        };
+        if (p.pre) {
+          put(bx, v);
+          if constexpr (kGlu) put(bx + kOutBox, u);
+        }
+        if constexpr (kGlu) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = act_value<MXB_ACT_SILU>(v[j]) * u[j];
+        } else {
+          act_apply(p.act, v);
+        }
+        if (p.residual && r < rows) {
+          const uint8_t* src = p.residual + (row * p.residual_ld + n) * 2;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (n + 8 * k < p.width) add8_bf16(v + 8 * k, *reinterpret_cast<const uint4*>(src + 16 * k));
+        }
+        if (p.c) put(bx + n_pre * kOutBox, v);
+        if (p.c_codes && r < rows) {
+          uint32_t w[16], q[4], byte;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) w[j] = cvt_bf16x2(v[2 * j], v[2 * j + 1]);
+          quant_block32<true>(w, QuantParams{1e-10f, -6.0f, 6.0f}, q, byte);
+          *reinterpret_cast<uint4*>(p.c_codes + (row * p.width + n) / 2) =
+              make_uint4(q[0], q[1], q[2], q[3]);
+          p.c_scales[(row * p.width + n) / 32] = (uint8_t)byte;
+        }
+        if (whole) fence_proxy_async_smem();
+        named_sync(1 + half, 128);
+        if (whole) {
+          if (issuer) {
+            if (p.pre) tma_store_2d(&map_pre, n, tl.m0, bx);
+            if (kGlu && p.pre) tma_store_2d(&map_pre_up, n, tl.m0, bx + kOutBox);
+            if (p.c) tma_store_2d(&map_c, n, tl.m0, bx + n_pre * kOutBox);
+          }
+        } else {
+          // the group's last rows: only they are written
+          auto copy = [&](const uint8_t* box, uint8_t* out, int64_t ld) {
+            for (int x = ht; x < rows * 4; x += 128) {
+              const int rr = x >> 2, k = x & 3;
+              if (n + 8 * k < p.width)
+                *reinterpret_cast<uint4*>(out + (((int64_t)tl.m0 + rr) * ld + n + 8 * k) * 2) =
+                    *reinterpret_cast<const uint4*>(box + rr * 64 + ((k ^ ((rr >> 1) & 3)) << 4));
+            }
+          };
+          if (p.pre) {
+            copy(bx, p.pre, p.pre_ld);
+            if (kGlu) copy(bx + kOutBox, p.pre + (int64_t)p.width * 2, p.pre_ld);
+          }
+          if (p.c) copy(bx + n_pre * kOutBox, p.c, p.c_ld);
+        }
+        if (issuer) bulk_commit();  // an empty group where nothing was stored
+        set = set + 1 == sets ? 0 : set + 1;
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty);
+    }
+    if (issuer) bulk_wait_all();
+  } else {
+    // ------------------------------------------------ A's scale bytes
+    const int q = warp - 10, r = q * 32 + lane;
+    const int mode = scale_mode(p);
+    uint2 next[4];
+    auto fetch = [&](const Tile& tl, int ks0) {
+      const int64_t row = (int64_t)tl.m0 + r;
+      const uint8_t* src = p.a_scales + row * p.a_spitch;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        next[j] = row < p.M && ks0 + j < ksteps ? row_scales(src, S, ks0 + j, mode)
+                                                : make_uint2(0u, 0u);
+    };
+    int gs = 0;
+    bool ok = true;
+    if (my_tiles > 0) fetch(tile_at(0), 0);
+    for (int i = 0; ok && i < my_tiles; ++i) {
+      const Tile tl = tile_at(i);
+      for (int ks0 = 0; ok && ks0 < ksteps; ks0 += 4) {
+        uint2 now[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) now[j] = next[j];
+        if (ks0 + 4 < ksteps) fetch(tl, ks0 + 4);
+        else if (i + 1 < my_tiles) fetch(tile_at(i + 1), 0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (ks0 + j >= ksteps) break;
+          const int s = gs % kWideStages;
+          if (gs >= kWideStages &&
+              !mbar_wait(&empty[s], (uint32_t)((gs / kWideStages - 1) & 1))) {
+            atomicExch(failed, 1);
+            ok = false;
+            break;
+          }
+          uint8_t* sf = smem + s * kWideStage + 3 * kBoxBytes + lane * 16 + q * 4;
+          *reinterpret_cast<uint32_t*>(sf) = now[j].x;
+          *reinterpret_cast<uint32_t*>(sf + 512) = now[j].y;
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[s]);
+          ++gs;
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+}
+
+// ---------------------------------------------------------------- narrow
+// The weights are the MMA's M side (kBlocks 128-row boxes: one, or gate and up)
+// and the kT rows its N side.  The CTAs of a cluster take consecutive ranges of
+// K; CTA r of the cluster owns the result columns n0 + r * 128 / size ...: every
+// CTA writes its partial accumulators into the owners' shared memory, and each
+// owner sums its columns over the ranks in order and runs the epilogue on them.
+//   warp 0       TMA of the weights' and rows' codes, the weights' scale atoms
+//   warp 1       MMA issue into one of two accumulators
+//   warps 2-5    accumulator -> owners, then sum + epilogue of the own columns
+//   warps 6, 7   the rows' scale bytes
+constexpr int kNarrowThreads = 256;
+
+template <bool kGlu, int kT>
+struct Narrow {
+  static constexpr int kBlocks = kGlu ? 2 : 1;
+  static constexpr uint32_t kStage =
+      kBlocks * (kBoxBytes + kAtoms) + (uint32_t)kT * 128 + kAtoms;
+  static constexpr uint32_t kPart = kBlocks * kT * 128 * 4;  // partial sums, all ranks
+  static constexpr size_t kFixed = 1024 + kPart + kGroupTableInts * 4 + 512;
+  static constexpr int kMost = (int)((227 * 1024 - kFixed) / kStage);
+  static constexpr int kStages = kMost > 9 ? 9 : kMost;
+  static constexpr size_t kSmem = kFixed + kStages * kStage;
+  static constexpr uint32_t kScaleCols = kBlocks * 8 + 8;
+  static_assert(kStages >= 3 && 2 * kBlocks * kT <= 256 && 256 + kStages * kScaleCols <= kTmemCols,
+                "the ring and tensor memory fit");
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+// The address of this CTA's shared-memory location in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void peer_store(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+__device__ __forceinline__ void peer_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void fence_cluster() {
+  asm volatile("fence.acq_rel.cluster;" ::: "memory");
+}
+// mbar_wait() on a barrier that other CTAs of the cluster arrive on.
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity) {
+  const uint32_t a = smem_addr(bar);
+  for (uint32_t i = 0; i < kWaitSpins; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n"
+        " mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(a), "r"(parity)
+        : "memory");
+    if (done) return true;
+  }
+  atomicAdd(&g_mxb_wait_timeouts, 1u);
+  return false;
+}
+
+template <bool kGlu, int kT>
+__global__ void __launch_bounds__(kNarrowThreads, 1) grouped_narrow_kernel(
+    const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+    const __grid_constant__ GroupedArgs p) {
+  using L = Narrow<kGlu, kT>;
+  constexpr int kBlocks = L::kBlocks, kStages = L::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  float* part = reinterpret_cast<float*>(smem + kStages * L::kStage);
+  uint64_t* full = reinterpret_cast<uint64_t*>(part + L::kPart / 4);
+  uint64_t* empty = full + kStages;
+  uint64_t* acc_full = empty + kStages;  // [2]
+  uint64_t* acc_empty = acc_full + 2;    // [2]
+  uint64_t* part_full = acc_empty + 2;
+  uint64_t* part_empty = part_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(part_empty + 1);
+  int* failed = reinterpret_cast<int*>(tmem_slot + 1);
+  GroupTable g;
+  g.off = failed + 1;
+  g.tile = g.off + p.E + 1;
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  const uint32_t rank = cluster_rank(), ranks = cluster_size();
+  const int ntn = (p.width + 127) / 128;
+  const int ksteps = (p.K + kStepK - 1) / kStepK;
+  const int k_begin = (int)((int64_t)ksteps * rank / ranks);
+  const int k_end = (int)((int64_t)ksteps * (rank + 1) / ranks);
+  const int S = p.K / 32, S4 = (S + 3) / 4;
+
+  if (warp == 0) {
+    build_groups(g, p.m_splits, p.E, p.M, [&](int rows) { return (rows + kT - 1) / kT * ntn; });
+  } else if (warp == 1) {
+    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_relinquish();
+  } else if (t == 64) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1 + (kT + 31) / 32);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 4);
+    }
+    mbar_init(part_full, ranks);
+    mbar_init(part_empty, ranks);
+    fence_mbar_init();
+    *failed = 0;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  cluster_sync();  // every CTA's barriers are ready for its peers
+  const uint32_t tmem = *tmem_slot;
+  const int tiles = g.tile[p.E];
+  const int cluster = (int)(blockIdx.x / ranks), clusters = (int)(gridDim.x / ranks);
+  const int my_tiles = cluster < tiles ? (tiles - 1 - cluster) / clusters + 1 : 0;
+
+  struct Tile {
+    int e, m0, n0;
+  };
+  // row blocks fastest: the tiles that read the same weights run side by side
+  auto tile_at = [&](int i) {
+    const int id = cluster + i * clusters;
+    Tile r;
+    r.e = find_group(g.tile, p.E, id);
+    const int local = id - g.tile[r.e];
+    const int ntm = (g.tile[r.e + 1] - g.tile[r.e]) / ntn;
+    r.m0 = g.off[r.e] + local % ntm * kT;
+    r.n0 = local / ntm * 128;
+    return r;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------ TMA producer
+    if (lane == 0) {
+      int issued = 0;
+      bool ok = true;
+      for (int i = 0; ok && i < my_tiles; ++i) {
+        const Tile tl = tile_at(i);
+        for (int ks = k_begin; ks < k_end; ++ks) {
+          const int gs = issued, s = gs % kStages;
+          if (gs >= kStages && !mbar_wait(&empty[s], (uint32_t)((gs / kStages - 1) & 1))) {
+            atomicExch(failed, 1);
+            ok = false;
+            break;
+          }
+          uint8_t* st = smem + s * L::kStage;
+          uint8_t* sf = st + kBlocks * kBoxBytes + kT * 128;
+          const uint32_t atoms = (uint32_t)min(2, S4 - 2 * ks) * 512;
+          mbar_arrive_expect_tx(&full[s], kBlocks * (kBoxBytes + atoms) + kT * 128);
+          const int kx = ks * (kStepK / 2);
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) {
+            tma_load_2d(st + b * kBoxBytes, &map_b, kx, (kBlocks * tl.e + b) * p.width + tl.n0,
+                        &full[s]);
+            bulk_load_1d(sf + b * kAtoms,
+                         p.b_scales +
+                             ((int64_t)((kBlocks * tl.e + b) * ntn + tl.n0 / 128) * S4 + 2 * ks) * 512,
+                         atoms, &full[s]);
+          }
+          tma_load_2d(st + kBlocks * kBoxBytes, &map_a, kx, tl.m0, &full[s]);
+          issued = gs + 1;
+        }
+      }
+      // do not leave while copies of this CTA are still landing
+      for (int gs = issued > kStages ? issued - kStages : 0; gs < issued; ++gs)
+        mbar_wait(&full[gs % kStages], (uint32_t)((gs / kStages) & 1));
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      bool ok = true;
+      int gs = 0;
+      for (int i = 0; ok && i < my_tiles; ++i) {
+        const int buf = i & 1;
+        if (i > 1 && !mbar_wait(&acc_empty[buf], (uint32_t)((i / 2 - 1) & 1))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        for (int ks = k_begin; ks < k_end; ++ks, ++gs) {
+          const int s = gs % kStages;
+          if (!mbar_wait(&full[s], (uint32_t)((gs / kStages) & 1))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint8_t* st = smem + s * L::kStage;
+          const uint8_t* sf = st + kBlocks * kBoxBytes + kT * 128;
+          const uint32_t sfw = tmem + kScaleCol + (uint32_t)s * L::kScaleCols;
+          const uint32_t sfr = sfw + kBlocks * 8;
+          const int left = p.K - ks * kStepK;
+#pragma unroll
+          for (int a = 0; a < 2; ++a) {
+            if (128 * a >= left) break;
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b)
+              tc_copy_sf(sfw + 8 * b + 4 * a, smem_desc_sf(sf + b * kAtoms + a * 512));
+            tc_copy_sf(sfr + 4 * a, smem_desc_sf(sf + kBlocks * kAtoms + a * 512));
+          }
+          const uint64_t dr = smem_desc_sw128(st + kBlocks * kBoxBytes);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (64 * j >= left) break;
+            const uint32_t sf_id = (uint32_t)(j & 1) * 2u;
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b)
+              tc_mma(tmem + (uint32_t)((buf * kBlocks + b) * kT),
+                     smem_desc_sw128(st + b * kBoxBytes) + (uint64_t)(2 * j),
+                     dr + (uint64_t)(2 * j), mxf4_idesc(kT, sf_id),
+                     (sfw + 8 * b + 4 * (j >> 1)) | (sf_id << 30),
+                     (sfr + 4 * (j >> 1)) | (sf_id << 30), (ks > k_begin || j > 0) ? 1u : 0u);
+          }
+          tc_commit(&empty[s]);
+        }
+        tc_commit(&acc_full[buf]);
+      }
+      if (!ok) atomicExch(failed, 1);
+    }
+  } else if (warp < 6) {
+    // ------------------------------------------------ exchange and epilogue
+    const int quad = warp & 3, et = t - 64;
+    const int cols = 128 / (int)ranks;  // result columns of an owner
+    const int n_acc = quad * 32 + lane;
+    const uint32_t to = peer_addr(smem_addr(part), (uint32_t)(n_acc / cols)) +
+                        (uint32_t)(((int)rank * kBlocks * kT * cols + n_acc % cols) * 4);
+    for (int i = 0; i < my_tiles; ++i) {
+      const Tile tl = tile_at(i);
+      const int rows = min(kT, g.off[tl.e + 1] - tl.m0);
+      const int buf = i & 1;
+      bool ok = mbar_wait(&acc_full[buf], (uint32_t)((i / 2) & 1));
+      // every owner has summed tile i - 1
+      if (i > 0) ok = mbar_wait_cluster(part_empty, (uint32_t)((i - 1) & 1)) && ok;
+      tc_fence_after();
+      if (!ok) atomicExch(failed, 1);
+      __syncwarp();
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+        for (int c = 0; c < kT; c += 16) {
+          uint32_t acc[16];
+          tmem_ld16(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)((buf * kBlocks + b) * kT + c),
+                    acc);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            peer_store(to + (uint32_t)((b * kT + c + j) * cols * 4), __uint_as_float(acc[j]));
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[buf]);
+      named_sync(1, 128);
+      if (et < (int)ranks) {
+        fence_cluster();
+        peer_arrive(peer_addr(smem_addr(part_full), (uint32_t)et));
+      }
+      __syncwarp();
+      ok = mbar_wait_cluster(part_full, (uint32_t)(i & 1));
+      if (!ok) atomicExch(failed, 1);
+      // a wait that gave up ends the tiles of this CTA; its peers give up in turn
+      if (named_sync_or(1, 128, !ok || *((volatile int*)failed))) break;
+      {
+        const int per_row = cols / 8;
+        for (int x = et; x < kT * per_row; x += 128) {
+          const int tr = x / per_row, c8 = x % per_row * 8;
+          const int n = tl.n0 + (int)rank * cols + c8;
+          float v[8], u[kGlu ? 8 : 1];
+          const bool in = tr < rows && n < p.width;
+          if (in) {
+            auto sum = [&](int b, float* z) {
+              const float* src = part + (b * kT + tr) * cols + c8;
+#pragma unroll
+              for (int k = 0; k < 8; ++k) z[k] = 0.0f;
+              for (int q = 0; q < (int)ranks; ++q, src += kBlocks * kT * cols) {
+                const float4 lo = *reinterpret_cast<const float4*>(src);
+                const float4 hi = *reinterpret_cast<const float4*>(src + 4);
+                z[0] += lo.x; z[1] += lo.y; z[2] += lo.z; z[3] += lo.w;
+                z[4] += hi.x; z[5] += hi.y; z[6] += hi.z; z[7] += hi.w;
+              }
+              if (p.bias) {
+                const int64_t at = (int64_t)(kBlocks * tl.e + b) * p.width + n;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) z[k] += load_bias(p, at + k);
+              }
+            };
+            const int64_t row = (int64_t)tl.m0 + tr;
+            sum(0, v);
+            if (p.pre)
+              *reinterpret_cast<uint4*>(p.pre + (row * p.pre_ld + n) * 2) = pack8_bf16(v);
+            if constexpr (kGlu) {
+              sum(1, u);
+              if (p.pre)
+                *reinterpret_cast<uint4*>(p.pre + (row * p.pre_ld + p.width + n) * 2) =
+                    pack8_bf16(u);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) v[k] = act_value<MXB_ACT_SILU>(v[k]) * u[k];
+            } else {
+              act_apply(p.act, v);
+            }
+            if (p.residual)
+              add8_bf16(v, *reinterpret_cast<const uint4*>(p.residual + (row * p.residual_ld + n) * 2));
+            if (p.c) *reinterpret_cast<uint4*>(p.c + (row * p.c_ld + n) * 2) = pack8_bf16(v);
+          }
+          if (p.c_codes)
+            quant_quad(p.c_codes, p.c_scales, v, in, ((int64_t)tl.m0 + tr) * p.width + n);
+        }
+      }
+      // the partial sums have been read
+      named_sync(1, 128);
+      if (et < (int)ranks) {
+        fence_cluster();
+        peer_arrive(peer_addr(smem_addr(part_empty), (uint32_t)et));
+      }
+      __syncwarp();
+    }
+  } else {
+    // ------------------------------------------------ the rows' scale bytes
+    const int r = (warp - 6) * 32 + lane;
+    if ((warp - 6) * 32 < kT) {
+      const int mode = scale_mode(p);
+      uint2 next[4];
+      auto fetch = [&](const Tile& tl, int ks0) {
+        const int64_t row = (int64_t)tl.m0 + r;
+        const uint8_t* src = p.a_scales + row * p.a_spitch;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          next[j] = r < kT && row < p.M && ks0 + j < k_end ? row_scales(src, S, ks0 + j, mode)
+                                                           : make_uint2(0u, 0u);
+      };
+      int gs = 0;
+      bool ok = true;
+      if (my_tiles > 0) fetch(tile_at(0), k_begin);
+      for (int i = 0; ok && i < my_tiles; ++i) {
+        const Tile tl = tile_at(i);
+        for (int ks0 = k_begin; ok && ks0 < k_end; ks0 += 4) {
+          uint2 now[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) now[j] = next[j];
+          if (ks0 + 4 < k_end) fetch(tl, ks0 + 4);
+          else if (i + 1 < my_tiles) fetch(tile_at(i + 1), k_begin);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (ks0 + j >= k_end) break;
+            const int s = gs % kStages;
+            if (gs >= kStages && !mbar_wait(&empty[s], (uint32_t)((gs / kStages - 1) & 1))) {
+              atomicExch(failed, 1);
+              ok = false;
+              break;
+            }
+            uint8_t* sf = smem + s * L::kStage + kBlocks * (kBoxBytes + kAtoms) + kT * 128 +
+                          lane * 16 + (warp - 6) * 4;
+            *reinterpret_cast<uint32_t*>(sf) = now[j].x;
+            *reinterpret_cast<uint32_t*>(sf + 512) = now[j].y;
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[s]);
+            ++gs;
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+  __syncwarp();
+  cluster_sync();  // no peer still writes to, or arrives in, this CTA's shared memory
+}
+
+// ---------------------------------------------------------------- scales
+// One thread per 4-byte word (4 scales of a row) of the tiled layout.
+__global__ void __launch_bounds__(256) swizzle_grouped_kernel(const uint8_t* __restrict__ scales,
+                                                              int64_t ranges, int64_t rows, int S,
+                                                              uint32_t* __restrict__ out) {
+  const int64_t rb = (rows + 127) / 128, S4 = (S + 3) / 4;
+  const int64_t words = ranges * rb * 128 * S4;
+  for (int64_t w = (int64_t)blockIdx.x * 256 + threadIdx.x; w < words;
+       w += (int64_t)gridDim.x * 256) {
+    // word w of the output: atom (range, row block, column of atoms), lane row, quarter
+    const int in_atom = (int)(w & 127);
+    const int64_t atom = w >> 7, c4 = atom % S4, block = atom / S4;
+    const int64_t range = block / rb, r = block % rb * 128 + (in_atom & 3) * 32 + (in_atom >> 2);
+    uint32_t v = 0;
+    if (r < rows) {
+      const uint8_t* src = scales + (range * rows + r) * S + c4 * 4;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c4 * 4 + i < S) v |= (uint32_t)src[i] << (8 * i);
+    }
+    out[w] = v;
+  }
+}
+
+// ---------------------------------------------------------------- host side
+// Which kernel, and how.  rows: row-tile height (128 = wide); ranks: CTAs that
+// split K.
+struct Plan {
+  int rows, ranks;
+  int64_t tiles;  // upper bound over all splits
+};
+
+int64_t most_tiles(int64_t M, int64_t E, int rows, int64_t ntn) {
+  const int64_t groups = std::min(E, M);  // groups with a row
+  return (groups + (M - groups) / rows) * ntn;
+}
+
+Plan grouped_plan(const GroupedArgs& p, bool glu) {
+  const int sms = sm_count();
+  const int64_t ksteps = cdiv(p.K, kStepK);
+  const int64_t wide = most_tiles(p.M, p.E, 128, cdiv(p.width, glu ? 128 : 256));
+  Plan r{128, 1, wide};
+  if (p.M > 96 * (int64_t)p.E && wide >= sms) return r;
+  r.rows = p.M <= 24 * (int64_t)p.E ? 16 : 64;
+  r.tiles = most_tiles(p.M, p.E, r.rows, cdiv(p.width, 128));
+  const int most = p.c_codes ? 4 : 8;  // a quantized block of 32 columns has one owner
+  while (r.ranks < most && r.tiles * r.ranks * 2 <= sms && ksteps >= r.ranks * 4) r.ranks *= 2;
+  return r;
+}
+
+template <bool kGlu>
+mxb_status launch_wide(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc,
+                       const CUtensorMap& tp, const CUtensorMap& tu, const GroupedArgs& p,
+                       const Plan& plan, cudaStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  MXB_REQUIRE(grant_smem((const void*)grouped_wide_kernel<kGlu>, kWideSmem, done), MXB_ERR_CUDA,
+              "grouped_gemm_mxfp4: cannot reserve shared memory");
+  const unsigned grid = (unsigned)std::min<int64_t>(plan.tiles, sm_count());
+  grouped_wide_kernel<kGlu><<<grid, kWideThreads, kWideSmem, s>>>(ta, tb, tc, tp, tu, p);
+  return launch_status("grouped_gemm_mxfp4");
+}
+
+template <bool kGlu, int kT>
+mxb_status launch_narrow(const CUtensorMap& ta, const CUtensorMap& tb, const GroupedArgs& p,
+                         const Plan& plan, cudaStream_t s) {
+  using L = Narrow<kGlu, kT>;
+  static std::atomic<uint64_t> done{0};
+  MXB_REQUIRE(grant_smem((const void*)grouped_narrow_kernel<kGlu, kT>, L::kSmem, done),
+              MXB_ERR_CUDA, "grouped_gemm_mxfp4: cannot reserve shared memory");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(std::min<int64_t>(plan.tiles, std::max(1, sm_count() / plan.ranks)) *
+                                plan.ranks));
+  cfg.blockDim = dim3(kNarrowThreads);
+  cfg.dynamicSmemBytes = L::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)plan.ranks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, grouped_narrow_kernel<kGlu, kT>, ta, tb, p);
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    set_error("grouped_gemm_mxfp4: CUDA launch failed: %s", cudaGetErrorString(e));
+    return MXB_ERR_CUDA;
+  }
+  return MXB_OK;
+}
+
+}  // namespace
+}  // namespace mxb
+
+using namespace mxb;
+
+extern "C" mxb_status mxb_swizzle_scales_grouped(const void* scales, int64_t E, int64_t N,
+                                                 int64_t S, int32_t parts, void* out,
+                                                 mxb_stream_t stream) {
+  MXB_REQUIRE(E >= 0 && N >= 0 && S >= 0 && S <= INT32_MAX && (parts == 1 || parts == 2) &&
+                  N % parts == 0,
+              MXB_ERR_INVALID_ARGUMENT,
+              "swizzle_scales_grouped: need parts 1 or 2 and N %% parts == 0 (N=%lld parts=%d)",
+              (long long)N, parts);
+  if (E == 0 || N == 0 || S == 0) return MXB_OK;
+  MXB_REQUIRE(scales && out, MXB_ERR_INVALID_ARGUMENT, "swizzle_scales_grouped: null pointer");
+  MXB_REQUIRE(aligned(out, 16), MXB_ERR_MISALIGNED,
+              "swizzle_scales_grouped: out must be 16-byte aligned");
+  const int64_t words = E * parts * cdiv(N / parts, 128) * 128 * cdiv(S, 4);
+  swizzle_grouped_kernel<<<(unsigned)std::min<int64_t>(cdiv(words, 256), 16 * kSMs), 256, 0,
+                           to_cuda(stream)>>>((const uint8_t*)scales, E * parts, N / parts, (int)S,
+                                              (uint32_t*)out);
+  return launch_status("swizzle_scales_grouped");
+}
+
+extern "C" mxb_status mxb_grouped_gemm_mxfp4(const void* a_codes, int64_t a_codes_pitch,
+                                             const void* a_scales, int64_t a_scales_pitch,
+                                             int64_t M, const int32_t* m_splits, int32_t E,
+                                             const void* b_codes, const void* b_scales, int64_t N,
+                                             int64_t K, const mxb_epilogue* ep, void* c,
+                                             mxb_stream_t stream) {
+  const char* const what = "grouped_gemm_mxfp4";
+  MXB_REQUIRE(ep, MXB_ERR_INVALID_ARGUMENT, "%s: null epilogue", what);
+  MXB_REQUIRE(ep->activation >= MXB_ACT_NONE && ep->activation <= MXB_ACT_SWIGLU,
+              MXB_ERR_INVALID_ARGUMENT, "%s: unknown activation %d", what, ep->activation);
+  const bool glu = ep->activation == MXB_ACT_SWIGLU;
+  const int64_t parts = glu ? 2 : 1;
+  MXB_REQUIRE(M >= 0 && M <= INT32_MAX && E >= 1 && E <= MXB_MAX_EXPERTS, MXB_ERR_INVALID_ARGUMENT,
+              "%s: need 0 <= M < 2^31 and 1 <= E <= %d (M=%lld E=%d)", what, MXB_MAX_EXPERTS,
+              (long long)M, E);
+  MXB_REQUIRE(N >= 0 && N % (8 * parts) == 0 && K >= 32 && K % 32 == 0 && K <= (1 << 24),
+              MXB_ERR_INVALID_ARGUMENT,
+              "%s: need N %% %d == 0, K %% 32 == 0 and 32 <= K <= 2^24 (N=%lld K=%lld)", what,
+              (int)(8 * parts), (long long)N, (long long)K);
+  MXB_REQUIRE((int64_t)E * N <= INT32_MAX - 512, MXB_ERR_INVALID_ARGUMENT,
+              "%s: need E * N < 2^31 (E=%d N=%lld)", what, E, (long long)N);
+  if (M == 0 || N == 0) return MXB_OK;
+  const int64_t W = N / parts;
+  MXB_REQUIRE(a_codes && a_scales && b_codes && b_scales && (m_splits || E == 1),
+              MXB_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  MXB_REQUIRE(c || ep->pre || ep->c_codes, MXB_ERR_INVALID_ARGUMENT, "%s: no output", what);
+  MXB_REQUIRE(!ep->c_codes == !ep->c_scales && (!ep->c_codes || W % 32 == 0),
+              MXB_ERR_INVALID_ARGUMENT,
+              "%s: a quantized result needs both c_codes and c_scales and a width %% 32 == 0", what);
+  MXB_REQUIRE(a_codes_pitch >= K / 2 && a_scales_pitch >= K / 32 && (!c || ep->c_ld >= W) &&
+                  (!ep->pre || ep->pre_ld >= N) && (!ep->residual || ep->residual_ld >= W),
+              MXB_ERR_INVALID_ARGUMENT, "%s: a pitch does not cover its row", what);
+  MXB_REQUIRE(aligned(a_codes, 16) && a_codes_pitch % 16 == 0 && aligned(b_codes, 16) &&
+                  aligned(b_scales, 16) && aligned(c, 16) && aligned(ep->pre, 16) &&
+                  aligned(ep->residual, 16) && aligned(ep->c_codes, 16),
+              MXB_ERR_MISALIGNED, "%s: operands must be 16-byte aligned", what);
+  MXB_REQUIRE((!c || ep->c_ld % 8 == 0) && (!ep->pre || ep->pre_ld % 8 == 0) &&
+                  (!ep->residual || ep->residual_ld % 8 == 0),
+              MXB_ERR_MISALIGNED, "%s: pitches of c, pre and residual must be multiples of 8", what);
+  MXB_REQUIRE(!ep->bias || aligned(ep->bias, ep->bias_f32 ? 4 : 2), MXB_ERR_MISALIGNED,
+              "%s: bias is not aligned to its elements", what);
+
+  GroupedArgs p;
+  p.a_scales = (const uint8_t*)a_scales;
+  p.a_spitch = a_scales_pitch;
+  p.b_scales = (const uint8_t*)b_scales;
+  p.m_splits = m_splits;
+  p.M = M;
+  p.E = E;
+  p.width = (int)W;
+  p.K = (int)K;
+  p.act = ep->activation;
+  p.bias = ep->bias;
+  p.bias_f32 = ep->bias_f32;
+  p.residual = (const uint8_t*)ep->residual;
+  p.residual_ld = ep->residual_ld;
+  p.pre = (uint8_t*)ep->pre;
+  p.pre_ld = ep->pre_ld;
+  p.c = (uint8_t*)c;
+  p.c_ld = ep->c_ld;
+  p.c_codes = (uint8_t*)ep->c_codes;
+  p.c_scales = (uint8_t*)ep->c_scales;
+  const Plan plan = grouped_plan(p, glu);
+  MXB_REQUIRE(plan.tiles <= INT32_MAX, MXB_ERR_INVALID_ARGUMENT, "%s: too many tiles", what);
+
+  const cudaStream_t s = to_cuda(stream);
+  CUtensorMap ta, tb;
+  if (!make_tensor_map_2d(&ta, a_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, M, K / 2, a_codes_pitch,
+                          128, (uint32_t)plan.rows, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !make_tensor_map_2d(&tb, b_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (int64_t)E * N, K / 2,
+                          K / 2, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B))
+    return MXB_ERR_CUDA;
+  if (plan.rows == 16)
+    return glu ? launch_narrow<true, 16>(ta, tb, p, plan, s)
+               : launch_narrow<false, 16>(ta, tb, p, plan, s);
+  if (plan.rows == 64)
+    return glu ? launch_narrow<true, 64>(ta, tb, p, plan, s)
+               : launch_narrow<false, 64>(ta, tb, p, plan, s);
+  // output maps are one part wide, so that a box never reaches into the other part
+  CUtensorMap tc = ta, tp = ta, tu = ta;
+  auto out_map = [&](CUtensorMap* m, void* base, int64_t ld) {
+    return make_tensor_map_2d(m, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, M, W, ld, 32, 128,
+                              CU_TENSOR_MAP_SWIZZLE_64B);
+  };
+  if ((c && !out_map(&tc, c, ep->c_ld)) || (ep->pre && !out_map(&tp, ep->pre, ep->pre_ld)) ||
+      (ep->pre && glu && !out_map(&tu, (uint8_t*)ep->pre + W * 2, ep->pre_ld)))
+    return MXB_ERR_CUDA;
+  return glu ? launch_wide<true>(ta, tb, tc, tp, tu, p, plan, s)
+             : launch_wide<false>(ta, tb, tc, tp, tu, p, plan, s);
+}

@@ -1,0 +1,417 @@
+// The experts' weight gradients (sm_100a): dw[e][n, k] = sum over the rows r of
+// expert e of dy[r, n] * x[r, k], dy in BF16 as autograd hands it over, x the
+// MXFP4 rows saved by the forward pass.
+//
+// The contraction runs over rows, the outer dimension of both operands, so both
+// are MN-major for the tensor core and neither is transposed in memory.  An
+// E2M1 value times 2^(e - 127) is exact in BF16: eight warps expand x's codes
+// into a BF16 tile in shared memory while the tensor core works on the tiles
+// before, and the product is kind::f16 (BF16 x BF16 -> f32).  The tile is 128
+// columns of x (the M side: half the expanding work of 256) by 256 columns of
+// dy, 64 rows a step.
+//
+// Ragged groups: a step's rows past its expert's end are expanded as zeros, and
+// the same rows of dy (the next expert's, whatever they hold) are overwritten
+// with zeros in shared memory, so that an infinity or NaN there cannot reach
+// this expert's sums.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+
+#include "capi_util.h"
+#include "common.cuh"
+#include "groups.cuh"
+#include "host_util.h"
+#include "tma.cuh"
+#include "umma.cuh"
+
+namespace mxb {
+namespace {
+
+constexpr int kWgThreads = 448;  // TMA, MMA, 4 epilogue warps, 8 expanding warps
+constexpr int kWgStages = 4;
+constexpr int kWgRows = 64;                      // rows per step
+constexpr int kTileX = 128, kTileY = 256;        // columns of x and of dy
+constexpr uint32_t kWgBox = kWgRows * 128;       // 64 rows x 64 bf16 columns
+constexpr uint32_t kWgStage = (kTileX + kTileY) / 64 * kWgBox;
+constexpr size_t kWgSmem = 1024 + kWgStages * kWgStage + kGroupTableInts * 4 + 256;
+static_assert(kWgSmem <= 227 * 1024, "one CTA per SM");
+
+struct WgradArgs {
+  const uint8_t* x_codes;
+  int64_t x_pitch;
+  const uint8_t* x_scales;
+  int64_t s_pitch;
+  const int32_t* m_splits;
+  int64_t M;
+  int E, N, K;
+  uint8_t* dw;
+  int accumulate;
+};
+
+// 32 codes (16 bytes) and their E8M0 byte -> 32 BF16 values in element order:
+// e2m1 * 2^(e - 127) with one BF16 multiply by the power of two, whose BF16
+// pattern is e << 7 (exact; past BF16's range the product is infinite).  2^-127
+// has no normal pattern: e = 0 halves first and scales by 2^-126, also exact,
+// the result being a subnormal BF16.  e = 255 is the E8M0 NaN.
+__device__ __forceinline__ void expand32(uint4 codes, uint32_t e, uint32_t (&out)[16]) {
+  const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    e2m1x4_to_bf16x4(w[i], out[4 * i], out[4 * i + 1]);
+    e2m1x4_to_bf16x4(w[i] >> 16, out[4 * i + 2], out[4 * i + 3]);
+  }
+  uint32_t f = e == 255u ? 0x7FFFu : e << 7;
+  if (e == 0u) {  // 2^-127 = 2^-126 * 1/2: halve first (exact), then scale by 2^-126
+#pragma unroll
+    for (int i = 0; i < 16; ++i) out[i] = mul_bf16x2(out[i], 0x3F003F00u);
+    f = 1u << 7;
+  }
+  f |= f << 16;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) out[i] = mul_bf16x2(out[i], f);
+}
+
+template <bool kF32>
+__global__ void __launch_bounds__(kWgThreads, 1) grouped_wgrad_kernel(
+    const __grid_constant__ CUtensorMap map_dy, const __grid_constant__ WgradArgs p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  uint64_t* dy_full = reinterpret_cast<uint64_t*>(smem + kWgStages * kWgStage);
+  uint64_t* x_full = dy_full + kWgStages;
+  uint64_t* empty = x_full + kWgStages;
+  uint64_t* acc_full = empty + kWgStages;  // [2]
+  uint64_t* acc_empty = acc_full + 2;      // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  int* failed = reinterpret_cast<int*>(tmem_slot + 1);
+  GroupTable g;
+  g.off = failed + 1;
+  g.tile = g.off + p.E + 1;
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  const int nty = (p.N + kTileY - 1) / kTileY, ntx = (p.K + kTileX - 1) / kTileX;
+  const int per_expert = nty * ntx;
+
+  if (warp == 0) {
+    build_groups(g, p.m_splits, p.E, p.M, [&](int) { return 0; });
+  } else if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  } else if (t == 64) {
+    for (int s = 0; s < kWgStages; ++s) {
+      mbar_init(&dy_full[s], 1);
+      mbar_init(&x_full[s], 8);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 4);
+    }
+    fence_mbar_init();
+    *failed = 0;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int tiles = p.E * per_expert;
+  const int my_tiles =
+      (int)blockIdx.x < tiles ? (tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+
+  struct Tile {
+    int e, x0, y0, row0, rows, steps;
+  };
+  auto tile_at = [&](int i) {
+    const int id = (int)blockIdx.x + i * (int)gridDim.x;
+    Tile r;
+    r.e = id / per_expert;
+    const int local = id % per_expert;
+    r.x0 = local / nty * kTileX;
+    r.y0 = local % nty * kTileY;
+    r.row0 = g.off[r.e];
+    r.rows = g.off[r.e + 1] - r.row0;
+    r.steps = (r.rows + kWgRows - 1) / kWgRows;
+    return r;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------ TMA producer
+    if (lane == 0) {
+      int gs = 0;
+      bool ok = true;
+      for (int i = 0; ok && i < my_tiles; ++i) {
+        const Tile tl = tile_at(i);
+        for (int st = 0; st < tl.steps; ++st) {
+          const int s = gs % kWgStages;
+          if (gs >= kWgStages && !mbar_wait(&empty[s], (uint32_t)((gs / kWgStages - 1) & 1))) {
+            atomicExch(failed, 1);
+            ok = false;
+            break;
+          }
+          uint8_t* dst = smem + s * kWgStage + kTileX / 64 * kWgBox;
+          const int boxes = min(kTileY / 64, (p.N - tl.y0 + 63) / 64);
+          mbar_arrive_expect_tx(&dy_full[s], (uint32_t)boxes * kWgBox);
+          for (int b = 0; b < boxes; ++b)
+            tma_load_2d(dst + b * kWgBox, &map_dy, tl.y0 + 64 * b, tl.row0 + st * kWgRows,
+                        &dy_full[s]);
+          ++gs;
+        }
+      }
+      // do not leave while copies of this CTA are still landing
+      for (int q = gs > kWgStages ? gs - kWgStages : 0; q < gs; ++q)
+        mbar_wait(&dy_full[q % kWgStages], (uint32_t)((q / kWgStages) & 1));
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      bool ok = true;
+      int gs = 0;
+      for (int i = 0; ok && i < my_tiles; ++i) {
+        const int buf = i & 1, steps = tile_at(i).steps;
+        if (i > 1 && !mbar_wait(&acc_empty[buf], (uint32_t)((i / 2 - 1) & 1))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        for (int st = 0; st < steps; ++st, ++gs) {
+          const int s = gs % kWgStages;
+          const uint32_t ph = (uint32_t)((gs / kWgStages) & 1);
+          if (!mbar_wait(&dy_full[s], ph) || !mbar_wait(&x_full[s], ph)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t dx = smem_desc_mn_sw128(smem + s * kWgStage, kWgBox);
+          const uint64_t dyd =
+              smem_desc_mn_sw128(smem + s * kWgStage + kTileX / 64 * kWgBox, kWgBox);
+#pragma unroll
+          for (int j = 0; j < kWgRows / 16; ++j)  // 16 rows of 128 bytes further each
+            tc_mma_bf16(tmem + (uint32_t)(buf * kTileY), dx + (uint64_t)(128 * j),
+                        dyd + (uint64_t)(128 * j), bf16_mn_idesc(kTileY),
+                        (st > 0 || j > 0) ? 1u : 0u);
+          tc_commit(&empty[s]);
+        }
+        tc_commit(&acc_full[buf]);
+      }
+      if (!ok) atomicExch(failed, 1);
+    }
+  } else if (warp < 6) {
+    // ------------------------------------------------ epilogue: lane = column of x
+    const int quad = warp & 3;
+    for (int i = 0; i < my_tiles; ++i) {
+      const Tile tl = tile_at(i);
+      const int buf = i & 1;
+      const bool ok = mbar_wait(&acc_full[buf], (uint32_t)((i / 2) & 1));
+      tc_fence_after();
+      if (named_sync_or(1, 128, !ok || *((volatile int*)failed))) break;
+      const int k = tl.x0 + quad * 32 + lane;
+      const bool store = k < p.K && (tl.steps > 0 || !p.accumulate);
+#pragma unroll 1
+      for (int c = 0; c < kTileY; c += 32) {
+        if (tl.y0 + c >= p.N) break;
+        uint32_t acc[32];
+        __syncwarp();
+        tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * kTileY + c), acc);
+        tmem_ld_wait();
+        if (tl.steps == 0) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[j] = 0u;
+        }
+        const int64_t at = ((int64_t)tl.e * p.N + tl.y0 + c) * p.K + k;
+        if constexpr (kF32) {
+          float* out = reinterpret_cast<float*>(p.dw) + at;
+          if (store) {
+            if (p.accumulate) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (tl.y0 + c + j < p.N)
+                  acc[j] = __float_as_uint(__uint_as_float(acc[j]) + out[(int64_t)j * p.K]);
+            }
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (tl.y0 + c + j < p.N) out[(int64_t)j * p.K] = __uint_as_float(acc[j]);
+          }
+        } else {
+          // neighbouring lanes trade values of two columns of dy, so that each
+          // stores two neighbouring columns of x: 4-byte stores
+          const bool odd = lane & 1;
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const uint32_t give = odd ? acc[j] : acc[j + 1];
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, give, 1);
+            const float lo = __uint_as_float(odd ? got : acc[j]);
+            const float hi = __uint_as_float(odd ? acc[j + 1] : got);
+            const int n = tl.y0 + c + j + (odd ? 1 : 0);
+            if (store && n < p.N)
+              *reinterpret_cast<uint32_t*>(p.dw + (((int64_t)tl.e * p.N + n) * p.K + (k & ~1)) * 2) =
+                  cvt_bf16x2(lo, hi);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[buf]);
+    }
+  } else {
+    // ------------------------------------------------ x: MXFP4 -> BF16 tile
+    // Warp c has rows 8c .. 8c + 7 of a step, lane (b, r) the block of 32
+    // columns b of row r: 64 contiguous code bytes a row, and eight lanes of a
+    // 16-byte store phase in eight different rows, whose swizzled chunks are
+    // distinct.  The codes of the next kAhead steps are in registers.
+    constexpr int kAhead = 4;
+    const int c = warp - 6, b = lane >> 3, r = c * 8 + (lane & 7);
+    uint4 codes[kAhead];
+    uint32_t scale[kAhead];
+    int li = 0, lst = 0;  // tile and step of the next load
+    Tile lt = {};
+    auto skip_empty = [&] {
+      while (li < my_tiles) {
+        lt = tile_at(li);
+        if (lt.steps > 0) break;
+        ++li;
+      }
+    };
+    auto load = [&](uint4& q, uint32_t& e) {
+      q = make_uint4(0u, 0u, 0u, 0u);
+      e = 127u;
+      if (li >= my_tiles) return;
+      const int in = lst * kWgRows + r, k = lt.x0 + 32 * b;
+      if (in < lt.rows && k < p.K) {
+        const int64_t row = (int64_t)lt.row0 + in;
+        q = __ldg(reinterpret_cast<const uint4*>(p.x_codes + row * p.x_pitch + k / 2));
+        e = __ldg(p.x_scales + row * p.s_pitch + k / 32);
+      }
+      if (++lst == lt.steps) {
+        lst = 0;
+        ++li;
+        skip_empty();
+      }
+    };
+    skip_empty();
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) load(codes[j], scale[j]);
+    int gs = 0, i = 0, st = 0;
+    Tile tl = {};
+    auto next_tile = [&] {
+      while (i < my_tiles) {
+        tl = tile_at(i);
+        if (tl.steps > 0) break;
+        ++i;
+      }
+    };
+    next_tile();
+    bool ok = true;
+    while (ok && i < my_tiles) {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        if (i >= my_tiles) break;
+        const int s = gs % kWgStages;
+        if (gs >= kWgStages && !mbar_wait(&empty[s], (uint32_t)((gs / kWgStages - 1) & 1))) {
+          atomicExch(failed, 1);
+          ok = false;
+          break;
+        }
+        uint32_t v[16];
+        expand32(codes[j], scale[j], v);
+        uint8_t* box = smem + s * kWgStage + (b >> 1) * kWgBox + r * 128;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<uint4*>(box + ((((b & 1) * 4 + q) ^ (r & 7)) << 4)) =
+              make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+        load(codes[j], scale[j]);
+        const int here = tl.rows - st * kWgRows;  // rows of the expert in this step
+        if (here < kWgRows) {
+          if (!mbar_wait(&dy_full[s], (uint32_t)((gs / kWgStages) & 1))) {
+            atomicExch(failed, 1);
+            ok = false;
+            break;
+          }
+          if (r >= here) {  // a row's four lanes: one box of 64 columns each
+            uint8_t* dyr = smem + s * kWgStage + (kTileX / 64 + b) * kWgBox + r * 128;
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              *reinterpret_cast<uint4*>(dyr + 16 * q) = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&x_full[s]);
+        ++gs;
+        if (++st == tl.steps) {
+          st = 0;
+          ++i;
+          next_tile();
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+template <bool kF32>
+mxb_status launch_wgrad(const CUtensorMap& map, const WgradArgs& p, cudaStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  MXB_REQUIRE(grant_smem((const void*)grouped_wgrad_kernel<kF32>, kWgSmem, done), MXB_ERR_CUDA,
+              "grouped_wgrad_mxfp4: cannot reserve shared memory");
+  const int64_t tiles = (int64_t)p.E * cdiv(p.N, kTileY) * cdiv(p.K, kTileX);
+  MXB_REQUIRE(tiles <= INT32_MAX, MXB_ERR_INVALID_ARGUMENT, "grouped_wgrad_mxfp4: too many tiles");
+  const unsigned grid = (unsigned)std::min<int64_t>(tiles, sm_count());
+  grouped_wgrad_kernel<kF32><<<grid, kWgThreads, kWgSmem, s>>>(map, p);
+  return launch_status("grouped_wgrad_mxfp4");
+}
+
+}  // namespace
+}  // namespace mxb
+
+using namespace mxb;
+
+extern "C" mxb_status mxb_grouped_wgrad_mxfp4(const void* dy, int64_t dy_ld, const void* x_codes,
+                                              int64_t x_codes_pitch, const void* x_scales,
+                                              int64_t x_scales_pitch, int64_t M,
+                                              const int32_t* m_splits, int32_t E, int64_t N,
+                                              int64_t K, void* dw, int32_t dw_f32,
+                                              int32_t accumulate, mxb_stream_t stream) {
+  const char* const what = "grouped_wgrad_mxfp4";
+  MXB_REQUIRE(M >= 0 && M <= INT32_MAX && E >= 1 && E <= MXB_MAX_EXPERTS, MXB_ERR_INVALID_ARGUMENT,
+              "%s: need 0 <= M < 2^31 and 1 <= E <= %d (M=%lld E=%d)", what, MXB_MAX_EXPERTS,
+              (long long)M, E);
+  MXB_REQUIRE(N >= 0 && N <= INT32_MAX - 512 && N % 8 == 0 && K >= 0 && K <= INT32_MAX - 512 &&
+                  K % 32 == 0,
+              MXB_ERR_INVALID_ARGUMENT, "%s: need N %% 8 == 0 and K %% 32 == 0 (N=%lld K=%lld)",
+              what, (long long)N, (long long)K);
+  MXB_REQUIRE(!accumulate || dw_f32, MXB_ERR_UNSUPPORTED, "%s: only a float dw accumulates", what);
+  if (N == 0 || K == 0) return MXB_OK;
+  MXB_REQUIRE(dw && (m_splits || E == 1), MXB_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  MXB_REQUIRE(aligned(dw, 16), MXB_ERR_MISALIGNED, "%s: operands must be 16-byte aligned", what);
+  if (M == 0) {  // no expert has rows
+    if (!accumulate &&
+        cudaMemsetAsync(dw, 0, (size_t)E * N * K * (dw_f32 ? 4 : 2), to_cuda(stream)) != cudaSuccess)
+      return launch_status(what);
+    return MXB_OK;
+  }
+  MXB_REQUIRE(dy && x_codes && x_scales, MXB_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  MXB_REQUIRE(dy_ld >= N && x_codes_pitch >= K / 2 && x_scales_pitch >= K / 32,
+              MXB_ERR_INVALID_ARGUMENT, "%s: a pitch does not cover its row", what);
+  MXB_REQUIRE(aligned(dy, 16) && dy_ld % 8 == 0 && aligned(x_codes, 16) && x_codes_pitch % 16 == 0,
+              MXB_ERR_MISALIGNED, "%s: operands must be 16-byte aligned", what);
+  CUtensorMap map;
+  if (!make_tensor_map_2d(&map, dy, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, M, N, dy_ld, 64, kWgRows,
+                          CU_TENSOR_MAP_SWIZZLE_128B))
+    return MXB_ERR_CUDA;
+  WgradArgs p;
+  p.x_codes = (const uint8_t*)x_codes;
+  p.x_pitch = x_codes_pitch;
+  p.x_scales = (const uint8_t*)x_scales;
+  p.s_pitch = x_scales_pitch;
+  p.m_splits = m_splits;
+  p.M = M;
+  p.E = E;
+  p.N = (int)N;
+  p.K = (int)K;
+  p.dw = (uint8_t*)dw;
+  p.accumulate = accumulate;
+  return dw_f32 ? launch_wgrad<true>(map, p, to_cuda(stream))
+                : launch_wgrad<false>(map, p, to_cuda(stream));
+}

@@ -141,6 +141,10 @@ __device__ __forceinline__ void bulk_wait_read_all() {
 __device__ __forceinline__ void bulk_wait_read_1() {
   asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
 }
+// Waits until at most three committed bulk store groups are still reading shared memory.
+__device__ __forceinline__ void bulk_wait_read_3() {
+  asm volatile("cp.async.bulk.wait_group.read 3;" ::: "memory");
+}
 // Waits until every committed bulk store has completed.
 __device__ __forceinline__ void bulk_wait_all() {
   asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");

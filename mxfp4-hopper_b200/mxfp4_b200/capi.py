@@ -98,6 +98,29 @@ SIGNATURES.update({
     "mxb_ep_nccl_combine": [_P, _HP, _P, _P, _I64, _P, _P],
 })
 
+class Epilogue(ctypes.Structure):
+    """mxb_epilogue of include/mxfp4_b200.h."""
+    _fields_ = [("bias", ctypes.c_void_p), ("bias_f32", ctypes.c_int32),
+                ("activation", ctypes.c_int32), ("residual", ctypes.c_void_p),
+                ("residual_ld", ctypes.c_int64), ("pre", ctypes.c_void_p),
+                ("pre_ld", ctypes.c_int64), ("c_ld", ctypes.c_int64),
+                ("c_codes", ctypes.c_void_p), ("c_scales", ctypes.c_void_p)]
+
+
+# mxb_activation
+ACTIVATIONS = {"none": 0, "relu": 1, "relu2": 2, "silu": 3, "gelu": 4, "gelu_tanh": 5, "swiglu": 6}
+
+_EP = ctypes.POINTER(Epilogue)
+SIGNATURES.update({
+    "mxb_swizzle_scales_grouped": [_P, _I64, _I64, _I64, _I32, _P, _P],
+    "mxb_grouped_gemm_mxfp4": [_P, _I64, _P, _I64, _I64, _P, _I32, _P, _P, _I64, _I64, _EP, _P, _P],
+    "mxb_grouped_wgrad_mxfp4": [_P, _I64, _P, _I64, _P, _I64, _I64, _P, _I32, _I64, _I64, _P, _I32,
+                                _I32, _P],
+    "mxb_bias_act_grad": [_P, _P, _I64, _P, _I32, _I64, _I32, _P, _P, _P, _P, _P, _I64, _P],
+    "mxb_moe_unpermute": [_P, _I64, _I64, _P, _I64, _I32, _P, _I64, _P, _P],
+    "mxb_moe_unpermute_grad": [_P, _P, _I64, _I64, _P, _I64, _I32, _P, _I64, _P, _P, _P, _P, _P],
+})
+
 STATUS = {0: "MXB_OK", 1: "MXB_ERR_INVALID_ARGUMENT", 2: "MXB_ERR_MISALIGNED", 3: "MXB_ERR_CUDA",
           4: "MXB_ERR_UNSUPPORTED"}
 
@@ -132,6 +155,8 @@ def load() -> ctypes.CDLL:
         L.mxb_gemm_wait_timeouts.restype = ctypes.c_uint
         L.mxb_ep_nccl_workspace_bytes.argtypes = [_I64, _I32, _I32, _I32]
         L.mxb_ep_nccl_workspace_bytes.restype = ctypes.c_int64
+        L.mxb_bias_act_grad_workspace.argtypes = [_I64, _I32, _I64]
+        L.mxb_bias_act_grad_workspace.restype = ctypes.c_int64
         L.mxb_quant_mxfp4_rowcol_host_workspace.argtypes = [_I64, _I64, _I64]
         L.mxb_quant_mxfp4_rowcol_host_workspace.restype = ctypes.c_int64
         _lib = L
@@ -157,7 +182,7 @@ def last_error() -> str:
 
 def wait_timeouts() -> int:
     """Bounded waits that gave up on the current device, over every kernel
-    that waits on an mbarrier (quantizers, column converters, GEMM)."""
+    that waits on an mbarrier (quantizers, column converters, GEMM, grouped products)."""
     return int(load().mxb_wait_timeouts())
 
 

@@ -445,6 +445,223 @@ void omo_gemm_mxfp4(at::Tensor a_codes, at::Tensor a_scales_swizzled, at::Tensor
                "omo_gemm_mxfp4");
 }
 
+// ---- MXFP4 experts (no reference counterpart)
+
+using OptTensor = c10::optional<at::Tensor>;
+
+// Row-major rows at any pitch: the last dimension contiguous.
+void check_rows(const at::Tensor& x, const char* name, int64_t rows, int64_t cols,
+                at::ScalarType st, const at::Tensor& like) {
+  TORCH_CHECK(x.is_cuda() && x.device() == like.device(), name, " must be on ", like.device());
+  check_dtype(x, st, name);
+  TORCH_CHECK(x.dim() == 2 && x.size(0) == rows && x.size(1) == cols, name, " must be [", rows,
+              ", ", cols, "], got ", x.sizes());
+  TORCH_CHECK((x.stride(1) == 1 || cols <= 1) && (x.stride(0) >= cols || rows <= 1), name,
+              " must have contiguous rows");
+}
+int64_t pitch(const at::Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
+
+void check_dense(const at::Tensor& x, const char* name, at::IntArrayRef sizes, at::ScalarType st,
+                 const at::Tensor& like) {
+  TORCH_CHECK(x.is_cuda() && x.device() == like.device(), name, " must be on ", like.device());
+  check_dtype(x, st, name);
+  TORCH_CHECK(x.sizes() == sizes && x.is_contiguous(), name, " must be a contiguous ", sizes,
+              ", got ", x.sizes());
+}
+
+const int32_t* check_splits(const OptTensor& m_splits, int64_t E, const at::Tensor& like) {
+  if (!m_splits) {
+    TORCH_CHECK(E == 1, "m_splits is needed for more than one expert");
+    return nullptr;
+  }
+  check_dense(*m_splits, "m_splits", {E}, at::kInt, like);
+  return (const int32_t*)m_splits->data_ptr();
+}
+void* opt_ptr(const OptTensor& x) { return x ? x->data_ptr() : nullptr; }
+
+void omo_swizzle_scales_grouped(at::Tensor scales, int64_t parts, at::Tensor out) {
+  OmoRange nvtx_range("omo_swizzle_scales_grouped");
+  OMO_CHECK_INPUT(scales);
+  check_dtype(scales, at::kByte, "scales");
+  TORCH_CHECK(scales.dim() == 3, "scales must be [E, N, K/32]");
+  TORCH_CHECK(parts == 1 || parts == 2, "parts must be 1 or 2");
+  const int64_t E = scales.size(0), N = scales.size(1), S = scales.size(2);
+  TORCH_CHECK(N % parts == 0, "N must be a multiple of parts");
+  check_dense(out, "out", {E, parts * ((N / parts + 127) / 128 * 128), (S + 3) / 4 * 4}, at::kByte,
+              scales);
+  c10::cuda::CUDAGuard g(scales.device());
+  check_status(mxb_swizzle_scales_grouped(scales.data_ptr(), E, N, S, (int32_t)parts,
+                                          out.data_ptr(), cur_stream()),
+               "omo_swizzle_scales_grouped");
+}
+
+void omo_grouped_gemm_mxfp4(at::Tensor a_codes, at::Tensor a_scales, OptTensor m_splits,
+                            at::Tensor b_codes, at::Tensor b_scales, OptTensor c, OptTensor bias,
+                            int64_t activation, OptTensor residual, OptTensor pre,
+                            OptTensor c_codes, OptTensor c_scales) {
+  OmoRange nvtx_range("omo_grouped_gemm_mxfp4");
+  OMO_CHECK_INPUT(b_codes);
+  check_dtype(b_codes, at::kByte, "b_codes");
+  TORCH_CHECK(b_codes.dim() == 3, "b_codes must be [E, N, K/2]");
+  TORCH_CHECK(a_codes.dim() == 2, "a_codes must be [M, K/2]");
+  TORCH_CHECK(activation >= MXB_ACT_NONE && activation <= MXB_ACT_SWIGLU, "unknown activation");
+  const int64_t E = b_codes.size(0), N = b_codes.size(1), K = b_codes.size(2) * 2;
+  const int64_t M = a_codes.size(0), parts = activation == MXB_ACT_SWIGLU ? 2 : 1, W = N / parts;
+  TORCH_CHECK(E >= 1 && N % parts == 0 && K % 32 == 0, "b_codes must be [E, N, K/2] with K % 32 == 0");
+  check_rows(a_codes, "a_codes", M, K / 2, at::kByte, b_codes);
+  check_rows(a_scales, "a_scales", M, K / 32, at::kByte, b_codes);
+  check_dense(b_scales, "b_scales", {E, parts * ((W + 127) / 128 * 128), (K / 32 + 3) / 4 * 4},
+              at::kByte, b_codes);
+  mxb_epilogue ep = {};
+  ep.activation = (int32_t)activation;
+  if (bias) {
+    ep.bias_f32 = bias->scalar_type() == at::kFloat;
+    check_dense(*bias, "bias", {E, N}, ep.bias_f32 ? at::kFloat : at::kBFloat16, b_codes);
+    ep.bias = bias->data_ptr();
+  }
+  if (residual) {
+    check_rows(*residual, "residual", M, W, at::kBFloat16, b_codes);
+    ep.residual = residual->data_ptr();
+    ep.residual_ld = pitch(*residual);
+  }
+  if (pre) {
+    check_rows(*pre, "pre", M, N, at::kBFloat16, b_codes);
+    ep.pre = pre->data_ptr();
+    ep.pre_ld = pitch(*pre);
+  }
+  if (c) {
+    check_rows(*c, "c", M, W, at::kBFloat16, b_codes);
+    ep.c_ld = pitch(*c);
+  }
+  TORCH_CHECK(c_codes.has_value() == c_scales.has_value(), "c_codes and c_scales go together");
+  if (c_codes) {
+    TORCH_CHECK(W % 32 == 0, "a quantized result needs a width that is a multiple of 32");
+    check_dense(*c_codes, "c_codes", {M, W / 2}, at::kByte, b_codes);
+    check_dense(*c_scales, "c_scales", {M, W / 32}, at::kByte, b_codes);
+    ep.c_codes = c_codes->data_ptr();
+    ep.c_scales = c_scales->data_ptr();
+  }
+  const int32_t* splits = check_splits(m_splits, E, b_codes);
+  c10::cuda::CUDAGuard g(b_codes.device());
+  check_status(mxb_grouped_gemm_mxfp4(a_codes.data_ptr(), pitch(a_codes), a_scales.data_ptr(),
+                                      pitch(a_scales), M, splits, (int32_t)E, b_codes.data_ptr(),
+                                      b_scales.data_ptr(), N, K, &ep, opt_ptr(c), cur_stream()),
+               "omo_grouped_gemm_mxfp4");
+}
+
+void omo_grouped_wgrad_mxfp4(at::Tensor dy, at::Tensor x_codes, at::Tensor x_scales,
+                             OptTensor m_splits, at::Tensor dw, bool accumulate) {
+  OmoRange nvtx_range("omo_grouped_wgrad_mxfp4");
+  OMO_CHECK_INPUT(dw);
+  TORCH_CHECK(dw.dim() == 3, "dw must be [E, N, K]");
+  const bool f32 = dw.scalar_type() == at::kFloat;
+  check_dtype(dw, f32 ? at::kFloat : at::kBFloat16, "dw");
+  TORCH_CHECK(dy.dim() == 2, "dy must be [M, N]");
+  const int64_t E = dw.size(0), N = dw.size(1), K = dw.size(2), M = dy.size(0);
+  TORCH_CHECK(E >= 1 && K % 32 == 0, "dw must be [E, N, K] with K % 32 == 0");
+  check_rows(dy, "dy", M, N, at::kBFloat16, dw);
+  check_rows(x_codes, "x_codes", M, K / 2, at::kByte, dw);
+  check_rows(x_scales, "x_scales", M, K / 32, at::kByte, dw);
+  const int32_t* splits = check_splits(m_splits, E, dw);
+  c10::cuda::CUDAGuard g(dw.device());
+  check_status(mxb_grouped_wgrad_mxfp4(dy.data_ptr(), pitch(dy), x_codes.data_ptr(),
+                                       pitch(x_codes), x_scales.data_ptr(), pitch(x_scales), M,
+                                       splits, (int32_t)E, N, K, dw.data_ptr(), f32 ? 1 : 0,
+                                       accumulate ? 1 : 0, cur_stream()),
+               "omo_grouped_wgrad_mxfp4");
+}
+
+int64_t omo_bias_act_grad_workspace(int64_t M, int64_t E, int64_t N) {
+  return mxb_bias_act_grad_workspace(M, (int32_t)E, N);
+}
+
+void omo_bias_act_grad(at::Tensor dy, OptTensor pre, OptTensor m_splits, int64_t E, int64_t N,
+                       int64_t activation, OptTensor dz, OptTensor dz_codes, OptTensor dz_scales,
+                       OptTensor dbias, OptTensor workspace) {
+  OmoRange nvtx_range("omo_bias_act_grad");
+  OMO_CHECK_INPUT(dy);
+  TORCH_CHECK(dy.dim() == 2, "dy must be [M, W]");
+  TORCH_CHECK(activation >= MXB_ACT_NONE && activation <= MXB_ACT_SWIGLU, "unknown activation");
+  TORCH_CHECK(E >= 1 && E <= MXB_MAX_EXPERTS, "need 1 <= E <= ", MXB_MAX_EXPERTS);
+  const int64_t M = dy.size(0), parts = activation == MXB_ACT_SWIGLU ? 2 : 1;
+  TORCH_CHECK(N % parts == 0, "N must be even for swiglu");
+  check_dense(dy, "dy", {M, N / parts}, at::kBFloat16, dy);
+  TORCH_CHECK(pre || activation == MXB_ACT_NONE, "pre is needed for this activation");
+  if (pre) check_dense(*pre, "pre", {M, N}, at::kBFloat16, dy);
+  if (dz) check_dense(*dz, "dz", {M, N}, at::kBFloat16, dy);
+  TORCH_CHECK(dz_codes.has_value() == dz_scales.has_value(), "dz_codes and dz_scales go together");
+  if (dz_codes) {
+    TORCH_CHECK(N % (32 * parts) == 0, "a quantized dz needs N % ", 32 * parts, " == 0");
+    check_dense(*dz_codes, "dz_codes", {M, N / 2}, at::kByte, dy);
+    check_dense(*dz_scales, "dz_scales", {M, N / 32}, at::kByte, dy);
+  }
+  if (dbias) check_dense(*dbias, "dbias", {E, N}, at::kFloat, dy);
+  if (workspace)
+    TORCH_CHECK(workspace->is_cuda() && workspace->device() == dy.device() &&
+                    workspace->is_contiguous(),
+                "workspace must be a contiguous CUDA tensor beside dy");
+  const int32_t* splits = check_splits(m_splits, E, dy);
+  c10::cuda::CUDAGuard g(dy.device());
+  check_status(
+      mxb_bias_act_grad(dy.data_ptr(), opt_ptr(pre), M, splits, (int32_t)E, N, (int32_t)activation,
+                        opt_ptr(dz), opt_ptr(dz_codes), opt_ptr(dz_scales), (float*)opt_ptr(dbias),
+                        opt_ptr(workspace), workspace ? (int64_t)workspace->nbytes() : 0,
+                        cur_stream()),
+      "omo_bias_act_grad");
+}
+
+// map int32 [T, >= topk] (row pitch = its stride); topk from the weights, or all columns.
+int64_t check_map(const at::Tensor& map, const OptTensor& weight, int64_t topk,
+                  const at::Tensor& like) {
+  TORCH_CHECK(map.dim() == 2 && map.size(1) >= topk, "map must be [T, >= topk]");
+  check_rows(map, "map", map.size(0), map.size(1), at::kInt, like);
+  if (weight) check_dense(*weight, "weight", {map.size(0), topk}, at::kFloat, like);
+  return map.size(0) > 1 ? map.stride(0) : map.size(1);
+}
+
+void omo_moe_unpermute(at::Tensor y, at::Tensor map, OptTensor weight, int64_t topk,
+                       at::Tensor out) {
+  OmoRange nvtx_range("omo_moe_unpermute");
+  OMO_CHECK_INPUT(y);
+  check_dtype(y, at::kBFloat16, "y");
+  TORCH_CHECK(y.dim() == 2, "y must be [R, H]");
+  const int64_t ld = check_map(map, weight, topk, y), T = map.size(0);
+  check_dense(out, "out", {T, y.size(1)}, at::kBFloat16, y);
+  c10::cuda::CUDAGuard g(y.device());
+  check_status(mxb_moe_unpermute(y.data_ptr(), y.size(0), y.size(1), (const int32_t*)map.data_ptr(),
+                                 ld, (int32_t)topk, (const float*)opt_ptr(weight), T,
+                                 out.data_ptr(), cur_stream()),
+               "omo_moe_unpermute");
+}
+
+void omo_moe_unpermute_grad(at::Tensor dout, OptTensor y, int64_t rows, at::Tensor map,
+                            OptTensor weight, int64_t topk, OptTensor dy, OptTensor dy_codes,
+                            OptTensor dy_scales, OptTensor dweight) {
+  OmoRange nvtx_range("omo_moe_unpermute_grad");
+  OMO_CHECK_INPUT(dout);
+  check_dtype(dout, at::kBFloat16, "dout");
+  TORCH_CHECK(dout.dim() == 2 && dout.size(0) == map.size(0), "dout must be [T, H]");
+  const int64_t T = dout.size(0), H = dout.size(1);
+  const int64_t ld = check_map(map, weight, topk, dout);
+  TORCH_CHECK(y || !dweight, "y is needed for dweight");
+  if (y) check_dense(*y, "y", {rows, H}, at::kBFloat16, dout);
+  if (dy) check_dense(*dy, "dy", {rows, H}, at::kBFloat16, dout);
+  TORCH_CHECK(dy_codes.has_value() == dy_scales.has_value(), "dy_codes and dy_scales go together");
+  if (dy_codes) {
+    TORCH_CHECK(H % 32 == 0, "a quantized dy needs H % 32 == 0");
+    check_dense(*dy_codes, "dy_codes", {rows, H / 2}, at::kByte, dout);
+    check_dense(*dy_scales, "dy_scales", {rows, H / 32}, at::kByte, dout);
+  }
+  if (dweight) check_dense(*dweight, "dweight", {T, topk}, at::kFloat, dout);
+  c10::cuda::CUDAGuard g(dout.device());
+  check_status(mxb_moe_unpermute_grad(dout.data_ptr(), opt_ptr(y), rows, H,
+                                      (const int32_t*)map.data_ptr(), ld, (int32_t)topk,
+                                      (const float*)opt_ptr(weight), T, opt_ptr(dy),
+                                      opt_ptr(dy_codes), opt_ptr(dy_scales),
+                                      (float*)opt_ptr(dweight), cur_stream()),
+               "omo_moe_unpermute_grad");
+}
+
 }  // namespace
 
 PYBIND11_MODULE(omo, m) {
@@ -503,4 +720,30 @@ PYBIND11_MODULE(omo, m) {
   m.def("omo_gemm_mxfp4", &omo_gemm_mxfp4, "Block-scaled MXFP4 GEMM C = A . B^T (tcgen05)",
         py::arg("a_codes"), py::arg("a_scales_swizzled"), py::arg("b_codes"),
         py::arg("b_scales_swizzled"), py::arg("c"));
+  m.def("omo_swizzle_scales_grouped", &omo_swizzle_scales_grouped,
+        "E8M0 scales of stacked weights -> 128x4-tile layout per part", py::arg("scales"),
+        py::arg("parts"), py::arg("out"));
+  m.def("omo_grouped_gemm_mxfp4", &omo_grouped_gemm_mxfp4,
+        "MXFP4 products grouped by expert with bias / activation / residual (tcgen05)",
+        py::arg("a_codes"), py::arg("a_scales"), py::arg("m_splits"), py::arg("b_codes"),
+        py::arg("b_scales"), py::arg("c"), py::arg("bias") = py::none(),
+        py::arg("activation") = 0, py::arg("residual") = py::none(), py::arg("pre") = py::none(),
+        py::arg("c_codes") = py::none(), py::arg("c_scales") = py::none());
+  m.def("omo_grouped_wgrad_mxfp4", &omo_grouped_wgrad_mxfp4,
+        "Weight gradients grouped by expert from BF16 dy and MXFP4 x (tcgen05)", py::arg("dy"),
+        py::arg("x_codes"), py::arg("x_scales"), py::arg("m_splits"), py::arg("dw"),
+        py::arg("accumulate") = false);
+  m.def("omo_bias_act_grad_workspace", &omo_bias_act_grad_workspace,
+        "Workspace bytes of omo_bias_act_grad", py::arg("M"), py::arg("E"), py::arg("N"));
+  m.def("omo_bias_act_grad", &omo_bias_act_grad, "Gradient of the bias / activation epilogue",
+        py::arg("dy"), py::arg("pre"), py::arg("m_splits"), py::arg("E"), py::arg("N"),
+        py::arg("activation"), py::arg("dz") = py::none(), py::arg("dz_codes") = py::none(),
+        py::arg("dz_scales") = py::none(), py::arg("dbias") = py::none(),
+        py::arg("workspace") = py::none());
+  m.def("omo_moe_unpermute", &omo_moe_unpermute, "Weighted sum of expert rows per token",
+        py::arg("y"), py::arg("map"), py::arg("weight"), py::arg("topk"), py::arg("out"));
+  m.def("omo_moe_unpermute_grad", &omo_moe_unpermute_grad, "Gradient of omo_moe_unpermute",
+        py::arg("dout"), py::arg("y"), py::arg("rows"), py::arg("map"), py::arg("weight"),
+        py::arg("topk"), py::arg("dy") = py::none(), py::arg("dy_codes") = py::none(),
+        py::arg("dy_scales") = py::none(), py::arg("dweight") = py::none());
 }
