@@ -10,7 +10,8 @@
 // group's end are computed and not written.
 //
 // Two kernels, chosen by grouped_plan() below:
-//   wide    128 rows x 256 weight rows a tile: the rows are the MMA's M side.
+//   wide    256 rows x 256 weight rows a tile: the rows are the M side of MMAs
+//           that two CTAs share.
 //   narrow  16 or 64 rows x 128 (gated: 256) weight rows a tile: the weights are
 //           the M side, so that a few rows do not pay for 128.  A cluster of up
 //           to 8 CTAs splits K; the partial accumulators meet in distributed
@@ -47,31 +48,84 @@ struct GroupedArgs {
   uint8_t *pre, *c;
   int64_t pre_ld, c_ld;
   uint8_t *c_codes, *c_scales;
+  int a_scales_tma;  // A's scales have a tensor map
 };
 
-// The 8 scale bytes of one row's K step as two words (the two atoms of the
-// step); bytes past the row's K / 32 scales are zero.
-__device__ __forceinline__ uint2 row_scales(const uint8_t* row, int S, int ks, int mode) {
-  const int b0 = ks * 8;
-  uint2 w = make_uint2(0u, 0u);
-  if (mode == 8) return *reinterpret_cast<const uint2*>(row + b0);  // S % 8 == 0
-  if (mode == 4) {                                                   // S % 4 == 0
-    w.x = *reinterpret_cast<const uint32_t*>(row + b0);
-    if (b0 + 4 < S) w.y = *reinterpret_cast<const uint32_t*>(row + b0 + 4);
+// The rows' E8M0 bytes on their way to the tensor core: a thread has one row of
+// the tile and hands out its 8 bytes (the two words of its place in the step's two
+// atoms; zero past the row's S = K / 32 bytes) step by step.  Where the rows are
+// whole aligned words (K % 128 == 0 and a pitch of a multiple of 4) the next four
+// steps' words are in flight in registers; else each step's bytes are read when
+// they are due.
+template <typename TileAt>
+struct RowScales {
+  const GroupedArgs& p;
+  const TileAt& tile_at;
+  int r, begin, end, tiles;  // row in the tile, K steps, tiles of this CTA
+  bool words;
+  const uint8_t* src = nullptr;
+  bool in = false;
+  int ti = 0, ks = 0;
+  uint32_t next[8], now[8];
+
+  __device__ __forceinline__ void seek() {
+    ks = begin;
+    in = false;
+    if (ti < tiles && r >= 0) {
+      const int64_t row = (int64_t)tile_at(ti).m0 + r;
+      in = row < p.M;
+      src = p.a_scales + row * p.a_spitch;
+    }
+  }
+  __device__ __forceinline__ void fetch() {
+    const int S = p.K / 32;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int at = ks * 8 + 4 * j;
+      next[j] = 0u;
+      if (words && in && at < S && ks + (j >> 1) < end)
+        next[j] = __ldg(reinterpret_cast<const uint32_t*>(src + at));
+    }
+  }
+  __device__ __forceinline__ RowScales(const GroupedArgs& p_, const TileAt& tile_at_, int r_,
+                                       int begin_, int end_, int tiles_)
+      : p(p_), tile_at(tile_at_), r(r_), begin(begin_), end(end_), tiles(tiles_) {
+    words = ((reinterpret_cast<uintptr_t>(p.a_scales) | (uintptr_t)p.a_spitch |
+              (uintptr_t)(p.K / 32)) & 3) == 0;
+    seek();
+    fetch();
+  }
+  // Takes the next four steps; they are handed out by get(0) .. get(3).
+  __device__ __forceinline__ void advance() {
+    if (!words) {
+      bytes_src = src;
+      bytes_in = in;
+      bytes_ks = ks;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) now[j] = next[j];
+    ks += 4;
+    if (ks >= end) {
+      ++ti;
+      seek();
+    }
+    fetch();
+  }
+  __device__ __forceinline__ uint2 get(int j) const {
+    uint2 w = make_uint2(now[2 * j], now[2 * j + 1]);
+    if (!words && bytes_in) {
+      const int S = p.K / 32, b0 = (bytes_ks + j) * 8;
+      for (int i = 0; i < 4; ++i) {
+        if (b0 + i < S) w.x |= (uint32_t)bytes_src[b0 + i] << (8 * i);
+        if (b0 + 4 + i < S) w.y |= (uint32_t)bytes_src[b0 + 4 + i] << (8 * i);
+      }
+    }
     return w;
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (b0 + i < S) w.x |= (uint32_t)row[b0 + i] << (8 * i);
-    if (b0 + 4 + i < S) w.y |= (uint32_t)row[b0 + 4 + i] << (8 * i);
-  }
-  return w;
-}
-__device__ __forceinline__ int scale_mode(const GroupedArgs& p) {
-  const uintptr_t any = reinterpret_cast<uintptr_t>(p.a_scales) | (uintptr_t)p.a_spitch |
-                        (uintptr_t)(p.K / 32);
-  return (any & 7) == 0 ? 8 : (any & 3) == 0 ? 4 : 1;
-}
+  const uint8_t* bytes_src = nullptr;
+  bool bytes_in = false;
+  int bytes_ks = 0;
+};
 
 __device__ __forceinline__ float load_bias(const GroupedArgs& p, int64_t i) {
   return p.bias_f32 ? static_cast<const float*>(p.bias)[i]
@@ -79,142 +133,190 @@ __device__ __forceinline__ float load_bias(const GroupedArgs& p, int64_t i) {
 }
 
 // ---------------------------------------------------------------- wide
-// One persistent CTA per SM; a tile has 128 rows and two 128-row weight boxes:
-// columns n0 .. n0 + 255 of the result, or (gated) gate and up rows of columns
-// n0 .. n0 + 127.
-//   warp 0       TMA of A's and B's codes and bulk copies of B's scale atoms
-//   warp 1       MMA issue (scale atoms to tensor memory, 4 MMAs of K = 64)
-//   warps 2-9    epilogue: two groups of four warps, each with half the columns
-//   warps 10-13  A's scale bytes: one row a thread, the next four steps' bytes
-//                in registers before they are needed
-constexpr int kWideThreads = 448;
-constexpr int kWideStages = 3;
+// A persistent pair of CTAs (cta_group::2) per two SMs; a tile has 256 rows, 128
+// in each CTA, and 256 weight rows, of which each CTA holds 128: columns n0 ..
+// n0 + 255 of the result, or (gated) the gate and the up rows of columns n0 ..
+// n0 + 127.  Each operand byte crosses L2 -> shared memory once per 256 x 256
+// tile instead of once per 128 x 256.
+//   warp 0       TMA of this CTA's half of A's and B's codes, completing on CTA
+//                0's barrier
+//   warp 1       (CTA 0) MMA issue: four M = 256, N = 256, K = 64 a step
+//   warp 2       scales of four K steps at a time: a TMA box of 32 bytes of each
+//                of A's rows, bulk copies of B's atoms (both halves)
+//   warps 4-7    scales: each warp gathers its lane quadrant's words of a step
+//                from shared memory and writes them to the step's tensor memory
+//                columns with tcgen05.st, so that the tensor pipe carries MMAs
+//                only.  The scales have rings of their own, deeper than the
+//                codes': their path is longer (copy, shared memory, tensor
+//                memory).  Rows that TMA cannot take (a pitch that is not a
+//                multiple of 16) are read by these warps, a row a thread
+//   warps 8-15   epilogue: two groups of four warps, each with half the columns.
+//                The accumulator is read into registers at once and given back,
+//                so that the next tile's products run under the epilogue
+constexpr int kWideThreads = 512;
+constexpr int kWideStages = 4;
 constexpr uint32_t kBoxBytes = 128 * 128;  // 128 rows of 128 code bytes
 constexpr uint32_t kAtoms = 2 * 512;       // scale atoms of 128 rows and one K step
-constexpr uint32_t kWideStage = 3 * kBoxBytes + 3 * kAtoms;
+constexpr uint32_t kWideStage = 2 * kBoxBytes;
+constexpr int kSbStages = 2;               // shared-memory scales of four steps each:
+constexpr uint32_t kSbA = 128 * 32;        // A's 128 rows of 32 bytes,
+constexpr uint32_t kSbB = 4 * kAtoms;      // 8 atoms of each of B's halves
+constexpr uint32_t kSbStage = kSbA + 2 * kSbB;
+constexpr int kSfStages = 8;               // steps of scales in tensor memory
 constexpr uint32_t kOutBox = 128 * 64;     // 128 rows x 32 bf16 columns, 64-byte swizzle
 constexpr int kOutSlots = 4;               // per epilogue group
 constexpr uint32_t kScaleCol = 256;        // tensor memory: accumulator, then scales
 constexpr uint32_t kTmemCols = 512;
-constexpr size_t kWideSmem = 1024 + kWideStages * kWideStage + 2 * kOutSlots * kOutBox + 256 * 4 +
-                             kGroupTableInts * 4 + 128;
+constexpr size_t kWideSmem = 1024 + kWideStages * kWideStage + kSbStages * kSbStage +
+                             2 * kOutSlots * kOutBox + 256 * 4 + kGroupTableInts * 4 + 512;
 static_assert(kWideSmem <= 227 * 1024, "one CTA per SM");
+static_assert(kScaleCol + 24 * kSfStages <= kTmemCols, "scales fit beside the accumulator");
+static_assert(kWideStage % 1024 == 0, "swizzled boxes start on 1024 bytes");
+// Registers: 512 threads x 128 at launch = 128 x 64 + 128 x 96 + 256 x 176.  The
+// scale warps must not spill: a spilled load is waited for where it is issued.
+constexpr int kWideCopyRegs = 64, kWideScaleRegs = 96, kWideEpilogueRegs = 176;
 
-template <bool kGlu>
+template <int kAct>
 __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
     const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-    const __grid_constant__ CUtensorMap map_c, const __grid_constant__ CUtensorMap map_pre,
-    const __grid_constant__ CUtensorMap map_pre_up, const __grid_constant__ GroupedArgs p) {
+    const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_c,
+    const __grid_constant__ CUtensorMap map_pre, const __grid_constant__ CUtensorMap map_pre_up,
+    const __grid_constant__ GroupedArgs p) {
+  constexpr bool kGlu = kAct == MXB_ACT_SWIGLU;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
-  uint8_t* out_boxes = smem + kWideStages * kWideStage;
+  uint8_t* scales = smem + kWideStages * kWideStage;
+  uint8_t* out_boxes = scales + kSbStages * kSbStage;
   float* bias_s = reinterpret_cast<float*>(out_boxes + 2 * kOutSlots * kOutBox);
-  uint64_t* full = reinterpret_cast<uint64_t*>(bias_s + 256);
+  uint64_t* full = reinterpret_cast<uint64_t*>(bias_s + 256);  // CTA 0's: codes of both CTAs
   uint64_t* empty = full + kWideStages;
-  uint64_t* acc_full = empty + kWideStages;
-  uint64_t* acc_empty = acc_full + 1;
+  uint64_t* sb_full = empty + kWideStages;   // four steps' scales in shared memory
+  uint64_t* sb_empty = sb_full + kSbStages;
+  uint64_t* sf_full = sb_empty + kSbStages;  // CTA 0's: a step's scales in tensor memory
+  uint64_t* sf_empty = sf_full + kSfStages;
+  uint64_t* acc_full = sf_empty + kSfStages;
+  uint64_t* acc_empty = acc_full + 1;  // CTA 0's
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 1);
   int* failed = reinterpret_cast<int*>(tmem_slot + 1);
   GroupTable g;
   g.off = failed + 1;
   g.tile = g.off + p.E + 1;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  const int rank = (int)cluster_rank();
   constexpr int kTileN = kGlu ? 128 : 256;
   const int ntn = (p.width + kTileN - 1) / kTileN;
   const int ksteps = (p.K + kStepK - 1) / kStepK;
   const int S = p.K / 32, S4 = (S + 3) / 4;
 
   if (warp == 0) {
-    build_groups(g, p.m_splits, p.E, p.M, [&](int rows) { return (rows + 127) / 128 * ntn; });
+    build_groups(g, p.m_splits, p.E, p.M, [&](int rows) { return (rows + 255) / 256 * ntn; });
   } else if (warp == 1) {
-    tmem_alloc(tmem_slot, kTmemCols);
-    tmem_relinquish();
+    tmem_alloc_pair(tmem_slot, kTmemCols);
   } else if (t == 64) {
     for (int s = 0; s < kWideStages; ++s) {
-      mbar_init(&full[s], 1 + 4);
+      mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
+    for (int s = 0; s < kSbStages; ++s) {
+      mbar_init(&sb_full[s], 1);
+      mbar_init(&sb_empty[s], 4);
+    }
+    for (int s = 0; s < kSfStages; ++s) {
+      mbar_init(&sf_full[s], 8);
+      mbar_init(&sf_empty[s], 1);
+    }
     mbar_init(acc_full, 1);
-    mbar_init(acc_empty, 8);
+    mbar_init(acc_empty, 16);
     fence_mbar_init();
     *failed = 0;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  cluster_sync();
   const uint32_t tmem = *tmem_slot;
   const int tiles = g.tile[p.E];
-  const int my_tiles =
-      (int)blockIdx.x < tiles ? (tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+  const int pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;
+  const int my_tiles = pair < tiles ? (tiles - 1 - pair) / pairs + 1 : 0;
 
   struct Tile {
-    int e, m0, n0;
+    int e, m0, n0;  // m0: this CTA's first row
   };
   auto tile_at = [&](int i) {
-    const int id = (int)blockIdx.x + i * (int)gridDim.x;
+    const int id = pair + i * pairs;
     Tile r;
     r.e = find_group(g.tile, p.E, id);
     const int local = id - g.tile[r.e];
-    r.m0 = g.off[r.e] + local / ntn * 128;
+    r.m0 = g.off[r.e] + local / ntn * 256 + rank * 128;
     r.n0 = local % ntn * kTileN;
     return r;
   };
 
-  if (warp == 0) {
-    // ------------------------------------------------ TMA producer
-    if (lane == 0) {
-      const int nbp = (p.width + 127) / 128;  // 128-row scale blocks of a weight part
-      int issued = 0;
+  // columns 128 .. 255 of a plain tile may all lie past the result: then CTA 1's
+  // weight rows are not loaded and its stale codes make columns that are not written
+  auto has_second = [&](const Tile& tl) { return kGlu || tl.n0 + 128 < p.width; };
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideCopyRegs));
+    if (warp == 0 && lane == 0) {
+      // ------------------------------------------------ TMA producer
+      const uint32_t full0 = peer_addr(smem_addr(full), 0);
+      int gs = 0;
       bool ok = true;
       for (int i = 0; ok && i < my_tiles; ++i) {
         const Tile tl = tile_at(i);
-        int row0, row1, sb0, sb1;
-        bool second = true;
-        if (kGlu) {
-          row0 = 2 * tl.e * p.width + tl.n0;
-          row1 = row0 + p.width;
-          sb0 = 2 * tl.e * nbp + tl.n0 / 128;
-          sb1 = sb0 + nbp;
-        } else {
-          row0 = tl.e * p.width + tl.n0;
-          row1 = row0 + 128;
-          sb0 = tl.e * nbp + tl.n0 / 128;
-          sb1 = sb0 + 1;
-          second = tl.n0 + 128 < p.width;  // else: stale codes, columns that are not written
-        }
-        for (int ks = 0; ks < ksteps; ++ks) {
-          const int gs = issued, s = gs % kWideStages;
-          if (gs >= kWideStages &&
-              !mbar_wait(&empty[s], (uint32_t)((gs / kWideStages - 1) & 1))) {
+        const int row = kGlu ? (2 * tl.e + rank) * p.width + tl.n0
+                             : tl.e * p.width + tl.n0 + 128 * rank;
+        const bool second = has_second(tl);
+        for (int ks = 0; ks < ksteps; ++ks, ++gs) {
+          const int s = gs % kWideStages;
+          if (gs >= kWideStages && !mbar_wait(&empty[s], (uint32_t)((gs / kWideStages - 1) & 1))) {
             atomicExch(failed, 1);
             ok = false;
             break;
           }
           uint8_t* st = smem + s * kWideStage;
-          uint8_t* sf = st + 3 * kBoxBytes + kAtoms;
-          const uint32_t atoms = (uint32_t)min(2, S4 - 2 * ks) * 512;
-          mbar_arrive_expect_tx(&full[s],
-                                kBoxBytes + (kBoxBytes + atoms) * (second ? 2u : 1u));
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], (second ? 4 : 3) * kBoxBytes);
           const int kx = ks * (kStepK / 2);
-          tma_load_2d(st, &map_a, kx, tl.m0, &full[s]);
-          tma_load_2d(st + kBoxBytes, &map_b, kx, row0, &full[s]);
-          bulk_load_1d(sf, p.b_scales + ((int64_t)sb0 * S4 + 2 * ks) * 512, atoms, &full[s]);
-          if (second) {
-            tma_load_2d(st + 2 * kBoxBytes, &map_b, kx, row1, &full[s]);
-            bulk_load_1d(sf + kAtoms, p.b_scales + ((int64_t)sb1 * S4 + 2 * ks) * 512, atoms,
-                         &full[s]);
-          }
-          issued = gs + 1;
+          tma_load_2d_pair(st, &map_a, kx, tl.m0, full0 + 8 * s);
+          if (rank == 0 || second) tma_load_2d_pair(st + kBoxBytes, &map_b, kx, row, full0 + 8 * s);
         }
       }
-      // do not leave while copies of this CTA are still landing
-      for (int gs = issued > kWideStages ? issued - kWideStages : 0; gs < issued; ++gs)
-        mbar_wait(&full[gs % kWideStages], (uint32_t)((gs / kWideStages) & 1));
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------ MMA issuer
-    if (lane == 0) {
+      // do not leave while copies are still landing (CTA 0 waits for both CTAs' codes)
+      for (int q = gs > kWideStages ? gs - kWideStages : 0; rank == 0 && q < gs; ++q)
+        mbar_wait(&full[q % kWideStages], (uint32_t)((q / kWideStages) & 1));
+    } else if (warp == 2 && lane == 0) {
+      // ------------------------------------------------ scales, four steps a time
+      const int nbp = (p.width + 127) / 128;  // 128-row scale blocks of a weight part
+      int gq = 0;
+      bool ok = true;
+      for (int i = 0; ok && i < my_tiles; ++i) {
+        const Tile tl = tile_at(i);
+        const int block = (kGlu ? 2 : 1) * tl.e * nbp + tl.n0 / 128;
+        const uint8_t* src0 = p.b_scales + (int64_t)block * S4 * 512;
+        const uint8_t* src1 = src0 + (int64_t)(kGlu ? nbp : 1) * S4 * 512;
+        const bool second = has_second(tl);
+        for (int k4 = 0; k4 < S4; k4 += 8, ++gq) {
+          const int s = gq % kSbStages;
+          if (gq >= kSbStages && !mbar_wait(&sb_empty[s], (uint32_t)((gq / kSbStages - 1) & 1))) {
+            atomicExch(failed, 1);
+            ok = false;
+            break;
+          }
+          uint8_t* sb = scales + s * kSbStage;
+          const uint32_t atoms = (uint32_t)min(8, S4 - k4) * 512;
+          mbar_arrive_expect_tx(&sb_full[s], (p.a_scales_tma ? kSbA : 0) + (second ? 2 : 1) * atoms);
+          if (p.a_scales_tma) tma_load_2d(sb, &map_sa, 4 * k4, tl.m0, &sb_full[s]);
+          bulk_load_1d(sb + kSbA, src0 + k4 * 512, atoms, &sb_full[s]);
+          if (second) bulk_load_1d(sb + kSbA + kSbB, src1 + k4 * 512, atoms, &sb_full[s]);
+        }
+      }
+      for (int q = gq > kSbStages ? gq - kSbStages : 0; q < gq; ++q)
+        mbar_wait(&sb_full[q % kSbStages], (uint32_t)((q / kSbStages) & 1));
+    } else if (warp == 1 && rank == 0) {
+      // ------------------------------------------------ MMA issuer
+      const bool one = elect_one();
       bool ok = true;
       int gs = 0;
       for (int i = 0; ok && i < my_tiles; ++i) {
@@ -224,43 +326,108 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
         }
         tc_fence_after();
         for (int ks = 0; ks < ksteps; ++ks, ++gs) {
-          const int s = gs % kWideStages;
-          if (!mbar_wait(&full[s], (uint32_t)((gs / kWideStages) & 1))) {
+          const int s = gs % kWideStages, f = gs % kSfStages;
+          if (!mbar_wait(&sf_full[f], (uint32_t)((gs / kSfStages) & 1)) ||
+              !mbar_wait(&full[s], (uint32_t)((gs / kWideStages) & 1))) {
             ok = false;
             break;
           }
           tc_fence_after();
+          __syncwarp();
           const uint8_t* st = smem + s * kWideStage;
-          const uint8_t* sf = st + 3 * kBoxBytes;
-          const uint32_t sfc = tmem + kScaleCol + (uint32_t)(s * 24);
+          const uint32_t sfc = tmem + kScaleCol + (uint32_t)(f * 24);
           const int left = p.K - ks * kStepK;  // elements of K from this step on
-#pragma unroll
-          for (int a = 0; a < 2; ++a) {
-            if (128 * a >= left) break;
-            tc_copy_sf(sfc + 4 * a, smem_desc_sf(sf + a * 512));
-            tc_copy_sf(sfc + 8 + 8 * a, smem_desc_sf(sf + kAtoms + a * 512));
-            tc_copy_sf(sfc + 12 + 8 * a, smem_desc_sf(sf + 2 * kAtoms + a * 512));
-          }
           const uint64_t da = smem_desc_sw128(st);
           const uint64_t db = smem_desc_sw128(st + kBoxBytes);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if (64 * j >= left) break;
             const uint32_t sf_id = (uint32_t)(j & 1) * 2u;
-            tc_mma(tmem, da + (uint64_t)(2 * j), db + (uint64_t)(2 * j), mxf4_idesc(256, sf_id),
-                   (sfc + 4 * (j >> 1)) | (sf_id << 30), (sfc + 8 + 8 * (j >> 1)) | (sf_id << 30),
-                   (ks > 0 || j > 0) ? 1u : 0u);
+            tc_mma_pair(tmem, da + (uint64_t)(2 * j), db + (uint64_t)(2 * j),
+                        mxf4_idesc(256, 256, sf_id), (sfc + 4 * (j >> 1)) | (sf_id << 30),
+                        (sfc + 8 + 8 * (j >> 1)) | (sf_id << 30), (ks > 0 || j > 0) ? 1u : 0u, one);
           }
-          tc_commit(&empty[s]);
+          tc_commit_pair(&empty[s], one);
+          tc_commit_pair(&sf_empty[f], one);
         }
-        tc_commit(acc_full);
+        __syncwarp();
+        tc_commit_pair(acc_full, one);
       }
       if (!ok) atomicExch(failed, 1);
     }
-  } else if (warp < 10) {
+  } else if (warp < 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideScaleRegs));
+    // ------------------------------------------------ scales
+    const int q = warp - 4, r = q * 32 + lane;
+    const uint32_t sf_full0 = peer_addr(smem_addr(sf_full), 0);
+    const uint32_t col0 = tmem + ((uint32_t)(q * 32) << 16) + kScaleCol;
+    RowScales<decltype(tile_at)> rows(p, tile_at, r, 0, ksteps, p.a_scales_tma ? 0 : my_tiles);
+    int gs = 0, gq = 0;
+    bool ok = true;
+    for (int i = 0; ok && i < my_tiles; ++i) {
+      for (int ks0 = 0; ok && ks0 < ksteps; ks0 += 4, ++gq) {
+        const int sq = gq % kSbStages;
+        uint8_t* sb = scales + sq * kSbStage;
+        bool up = mbar_wait(&sb_full[sq], (uint32_t)((gq / kSbStages) & 1));
+        if (!p.a_scales_tma) {
+          rows.advance();
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<uint2*>(sb + r * 32 + j * 8) = rows.get(j);
+          up = !named_sync_or(3, 128, !up);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+          const int two = min(2, ksteps - ks0 - j);
+          if (two <= 0) break;
+          // a row's 16 bytes are two steps of two atoms; the four rows of a lane fill
+          // the atoms' four columns
+          uint4 ra[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            ra[c] = *reinterpret_cast<const uint4*>(sb + (32 * c + lane) * 32 + j * 8);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (h >= two) break;
+            const uint32_t a[8] = {h ? ra[0].z : ra[0].x, h ? ra[1].z : ra[1].x,
+                                   h ? ra[2].z : ra[2].x, h ? ra[3].z : ra[3].x,
+                                   h ? ra[0].w : ra[0].y, h ? ra[1].w : ra[1].y,
+                                   h ? ra[2].w : ra[2].y, h ? ra[3].w : ra[3].y};
+            // the columns of one K atom of B's two halves are neighbours
+            uint32_t b[16];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint4 w = *reinterpret_cast<const uint4*>(
+                  sb + kSbA + (k & 1) * kSbB + (2 * (j + h) + (k >> 1)) * 512 + lane * 16);
+              b[4 * k] = w.x; b[4 * k + 1] = w.y; b[4 * k + 2] = w.z; b[4 * k + 3] = w.w;
+            }
+            const int s = gs % kSfStages;
+            up = up && (gs < kSfStages ||
+                        mbar_wait(&sf_empty[s], (uint32_t)((gs / kSfStages - 1) & 1)));
+            tc_fence_after();
+            __syncwarp();
+            tmem_st8(col0 + (uint32_t)(s * 24), a);
+            tmem_st16(col0 + (uint32_t)(s * 24 + 8), b);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) peer_signal(sf_full0 + 8 * s);
+            ++gs;
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sb_empty[sq]);
+        if (!__all_sync(0xffffffffu, up)) {
+          atomicExch(failed, 1);
+          ok = false;
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWideEpilogueRegs));
     // ------------------------------------------------ epilogue
-    const int half = (warp - 2) >> 2, quad = warp & 3;
-    const int r = quad * 32 + lane, ht = (t - 64) & 127;
+    const int half = (warp - 8) >> 2, quad = warp & 3;
+    const int r = quad * 32 + lane, ht = t & 127;
     const bool issuer = ht == 0;
     uint8_t* boxes = out_boxes + half * kOutSlots * kOutBox;
     float* bias_h = bias_s + half * 128;
@@ -268,164 +435,136 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
     const int n_pre = p.pre ? (kGlu ? 2 : 1) : 0;
     const int n_box = n_pre + (p.c ? 1 : 0);
     const int sets = n_box == 3 ? 1 : n_box == 2 ? 2 : 4;
+    const uint32_t acc_empty0 = peer_addr(smem_addr(acc_empty), 0);
+    const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
     int set = 0;
     for (int i = 0; i < my_tiles; ++i) {
       const Tile tl = tile_at(i);
-      const int rows = min(128, g.off[tl.e + 1] - tl.m0);
-      const int nh = tl.n0 + half * kHalfN;  // first result column of this group
+      const int rows = min(128, g.off[tl.e + 1] - tl.m0);  // none or fewer: CTA 1's share
+      const int nh = tl.n0 + half * kHalfN;                // first result column of this group
+      float bias = 0.0f;
       if (p.bias) {
         // this group's 128 accumulator columns: 128 of z, or 64 gate and 64 up
         const int col = kGlu ? nh + (ht & 63) : nh + ht;
         const int64_t at = kGlu ? (int64_t)tl.e * 2 * p.width + (ht < 64 ? 0 : p.width) + col
                                 : (int64_t)tl.e * p.width + col;
-        bias_h[ht] = col < p.width ? load_bias(p, at) : 0.0f;
-      } else {
-        bias_h[ht] = 0.0f;
+        if (col < p.width) bias = load_bias(p, at);
       }
+      bias_h[ht] = bias;
       const bool ok = mbar_wait(acc_full, (uint32_t)(i & 1));
       tc_fence_after();
       const bool live = ok && !*((volatile int*)failed);
       if (named_sync_or(1 + half, 128, !live)) break;  // the four warps leave together
-      const bool whole = rows == 128;
-      const int64_t row = (int64_t)tl.m0 + r;
-#pragma unroll 1
-      for (int ch = 0; ch < kHalfN / 32; ++ch) {
-        const int n = nh + 32 * ch;
-        if (n >= p.width) break;
-        const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
-        uint32_t acc[32];
-        float v[32], u[kGlu ? 32 : 1];
-        __syncwarp();
-        tmem_ld32(lane_base + (uint32_t)(half * kHalfN + 32 * ch), acc);
-        tmem_ld_wait();
+      uint32_t acc[128];
+      __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(acc[j]) + bias_h[32 * ch + j];
-        if constexpr (kGlu) {
-          tmem_ld32(lane_base + (uint32_t)(128 + half * kHalfN + 32 * ch), acc);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) u[j] = __uint_as_float(acc[j]) + bias_h[64 + 32 * ch + j];
-        }
-        // the boxes of this set have been read by the stores issued `sets` chunks ago
-        if (issuer) {
-          if (sets == 1) bulk_wait_read_all();
-          else if (sets == 2) bulk_wait_read_1();
-          else bulk_wait_read_3();
-        }
-        named_sync(1 + half, 128);
-        uint8_t* bx = boxes + set * n_box * kOutBox;
-        auto put = [&](uint8_t* box, const float* x) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            *reinterpret_cast<uint4*>(box + r * 64 + ((k ^ ((r >> 1) & 3)) << 4)) =
-                pack8_bf16(x + 8 * k);
-        };
-        if (p.pre) {
-          put(bx, v);
-          if constexpr (kGlu) put(bx + kOutBox, u);
-        }
-        if constexpr (kGlu) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = act_value<MXB_ACT_SILU>(v[j]) * u[j];
-        } else {
-          act_apply(p.act, v);
-        }
-        if (p.residual && r < rows) {
-          const uint8_t* src = p.residual + (row * p.residual_ld + n) * 2;
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (n + 8 * k < p.width) add8_bf16(v + 8 * k, *reinterpret_cast<const uint4*>(src + 16 * k));
-        }
-        if (p.c) put(bx + n_pre * kOutBox, v);
-        if (p.c_codes && r < rows) {
-          uint32_t w[16], q[4], byte;
-#pragma unroll
-          for (int j = 0; j < 16; ++j) w[j] = cvt_bf16x2(v[2 * j], v[2 * j + 1]);
-          quant_block32<true>(w, QuantParams{1e-10f, -6.0f, 6.0f}, q, byte);
-          *reinterpret_cast<uint4*>(p.c_codes + (row * p.width + n) / 2) =
-              make_uint4(q[0], q[1], q[2], q[3]);
-          p.c_scales[(row * p.width + n) / 32] = (uint8_t)byte;
-        }
-        if (whole) fence_proxy_async_smem();
-        named_sync(1 + half, 128);
-        if (whole) {
-          if (issuer) {
-            if (p.pre) tma_store_2d(&map_pre, n, tl.m0, bx);
-            if (kGlu && p.pre) tma_store_2d(&map_pre_up, n, tl.m0, bx + kOutBox);
-            if (p.c) tma_store_2d(&map_c, n, tl.m0, bx + n_pre * kOutBox);
-          }
-        } else {
-          // the group's last rows: only they are written
-          auto copy = [&](const uint8_t* box, uint8_t* out, int64_t ld) {
-            for (int x = ht; x < rows * 4; x += 128) {
-              const int rr = x >> 2, k = x & 3;
-              if (n + 8 * k < p.width)
-                *reinterpret_cast<uint4*>(out + (((int64_t)tl.m0 + rr) * ld + n + 8 * k) * 2) =
-                    *reinterpret_cast<const uint4*>(box + rr * 64 + ((k ^ ((rr >> 1) & 3)) << 4));
-            }
-          };
-          if (p.pre) {
-            copy(bx, p.pre, p.pre_ld);
-            if (kGlu) copy(bx + kOutBox, p.pre + (int64_t)p.width * 2, p.pre_ld);
-          }
-          if (p.c) copy(bx + n_pre * kOutBox, p.c, p.c_ld);
-        }
-        if (issuer) bulk_commit();  // an empty group where nothing was stored
-        set = set + 1 == sets ? 0 : set + 1;
-      }
+      for (int k = 0; k < 4; ++k)
+        tmem_ld32(lane_base + (uint32_t)(kGlu ? (k >> 1) * 128 + half * 64 + (k & 1) * 32
+                                              : half * 128 + k * 32),
+                  acc + 32 * k);
+      tmem_ld_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(acc_empty);
-    }
-    if (issuer) bulk_wait_all();
-  } else {
-    // ------------------------------------------------ A's scale bytes
-    const int q = warp - 10, r = q * 32 + lane;
-    const int mode = scale_mode(p);
-    uint2 next[4];
-    auto fetch = [&](const Tile& tl, int ks0) {
+      if (lane == 0) peer_signal(acc_empty0);
+      if (rows <= 0) continue;
+      const bool whole = rows == 128;
       const int64_t row = (int64_t)tl.m0 + r;
-      const uint8_t* src = p.a_scales + row * p.a_spitch;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        next[j] = row < p.M && ks0 + j < ksteps ? row_scales(src, S, ks0 + j, mode)
-                                                : make_uint2(0u, 0u);
-    };
-    int gs = 0;
-    bool ok = true;
-    if (my_tiles > 0) fetch(tile_at(0), 0);
-    for (int i = 0; ok && i < my_tiles; ++i) {
-      const Tile tl = tile_at(i);
-      for (int ks0 = 0; ok && ks0 < ksteps; ks0 += 4) {
-        uint2 now[4];
+      for (int ch = 0; ch < kHalfN / 32; ++ch) {
+        const int n = nh + 32 * ch;
+        if (n < p.width) {
+          uint4 res[4];
+          if (p.residual) {
+            const uint8_t* src = p.residual + (row * p.residual_ld + n) * 2;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) now[j] = next[j];
-        if (ks0 + 4 < ksteps) fetch(tl, ks0 + 4);
-        else if (i + 1 < my_tiles) fetch(tile_at(i + 1), 0);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (ks0 + j >= ksteps) break;
-          const int s = gs % kWideStages;
-          if (gs >= kWideStages &&
-              !mbar_wait(&empty[s], (uint32_t)((gs / kWideStages - 1) & 1))) {
-            atomicExch(failed, 1);
-            ok = false;
-            break;
+            for (int k = 0; k < 4; ++k)
+              res[k] = r < rows && n + 8 * k < p.width
+                           ? *reinterpret_cast<const uint4*>(src + 16 * k)
+                           : make_uint4(0u, 0u, 0u, 0u);
           }
-          uint8_t* sf = smem + s * kWideStage + 3 * kBoxBytes + lane * 16 + q * 4;
-          *reinterpret_cast<uint32_t*>(sf) = now[j].x;
-          *reinterpret_cast<uint32_t*>(sf + 512) = now[j].y;
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&full[s]);
-          ++gs;
+          float v[32], u[kGlu ? 32 : 1];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(acc[32 * ch + j]) + bias_h[32 * ch + j];
+          if constexpr (kGlu) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              u[j] = __uint_as_float(acc[64 + 32 * ch + j]) + bias_h[64 + 32 * ch + j];
+          }
+          // the boxes of this set have been read by the stores issued `sets` chunks ago
+          if (issuer) {
+            if (sets == 1) bulk_wait_read_all();
+            else if (sets == 2) bulk_wait_read_1();
+            else bulk_wait_read_3();
+          }
+          named_sync(1 + half, 128);
+          uint8_t* bx = boxes + set * n_box * kOutBox;
+          auto put = [&](uint8_t* box, const float* x) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              *reinterpret_cast<uint4*>(box + r * 64 + ((k ^ ((r >> 1) & 3)) << 4)) =
+                  pack8_bf16(x + 8 * k);
+          };
+          if (p.pre) {
+            put(bx, v);
+            if constexpr (kGlu) put(bx + kOutBox, u);
+          }
+          if constexpr (kGlu) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = act_value<MXB_ACT_SILU>(v[j]) * u[j];
+          } else {
+            act_each<kAct>(v);
+          }
+          if (p.residual) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) add8_bf16(v + 8 * k, res[k]);
+          }
+          if (p.c) put(bx + n_pre * kOutBox, v);
+          if (p.c_codes && r < rows) {
+            uint32_t w[16], q[4], byte;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j] = cvt_bf16x2(v[2 * j], v[2 * j + 1]);
+            quant_block32<true>(w, QuantParams{1e-10f, -6.0f, 6.0f}, q, byte);
+            *reinterpret_cast<uint4*>(p.c_codes + (row * p.width + n) / 2) =
+                make_uint4(q[0], q[1], q[2], q[3]);
+            p.c_scales[(row * p.width + n) / 32] = (uint8_t)byte;
+          }
+          if (whole) fence_proxy_async_smem();
+          named_sync(1 + half, 128);
+          if (whole) {
+            if (issuer) {
+              if (p.pre) tma_store_2d(&map_pre, n, tl.m0, bx);
+              if (kGlu && p.pre) tma_store_2d(&map_pre_up, n, tl.m0, bx + kOutBox);
+              if (p.c) tma_store_2d(&map_c, n, tl.m0, bx + n_pre * kOutBox);
+            }
+          } else {
+            // the group's last rows: only they are written
+            auto copy = [&](const uint8_t* box, uint8_t* out, int64_t ld) {
+              for (int x = ht; x < rows * 4; x += 128) {
+                const int rr = x >> 2, k = x & 3;
+                if (n + 8 * k < p.width)
+                  *reinterpret_cast<uint4*>(out + (((int64_t)tl.m0 + rr) * ld + n + 8 * k) * 2) =
+                      *reinterpret_cast<const uint4*>(box + rr * 64 + ((k ^ ((rr >> 1) & 3)) << 4));
+              }
+            };
+            if (p.pre) {
+              copy(bx, p.pre, p.pre_ld);
+              if (kGlu) copy(bx + kOutBox, p.pre + (int64_t)p.width * 2, p.pre_ld);
+            }
+            if (p.c) copy(bx + n_pre * kOutBox, p.c, p.c_ld);
+          }
+          if (issuer) bulk_commit();  // an empty group where nothing was stored
+          set = set + 1 == sets ? 0 : set + 1;
         }
       }
     }
+    if (issuer) bulk_wait_all();
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+  cluster_sync();  // both CTAs' products and copies have completed
+  if (warp == 1) tmem_dealloc_pair(tmem, kTmemCols);
+  __syncwarp();
+  cluster_sync();
 }
 
 // ---------------------------------------------------------------- narrow
@@ -454,54 +593,6 @@ struct Narrow {
   static_assert(kStages >= 3 && 2 * kBlocks * kT <= 256 && 256 + kStages * kScaleCols <= kTmemCols,
                 "the ring and tensor memory fit");
 };
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::
-                   : "memory");
-}
-// The address of this CTA's shared-memory location in CTA `rank` of the cluster.
-__device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void peer_store(uint32_t addr, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
-}
-__device__ __forceinline__ void peer_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
-               : "memory");
-}
-__device__ __forceinline__ void fence_cluster() {
-  asm volatile("fence.acq_rel.cluster;" ::: "memory");
-}
-// mbar_wait() on a barrier that other CTAs of the cluster arrive on.
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity) {
-  const uint32_t a = smem_addr(bar);
-  for (uint32_t i = 0; i < kWaitSpins; ++i) {
-    uint32_t done;
-    asm volatile(
-        "{\n .reg .pred p;\n"
-        " mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-        " selp.u32 %0, 1, 0, p;\n}"
-        : "=r"(done)
-        : "r"(a), "r"(parity)
-        : "memory");
-    if (done) return true;
-  }
-  atomicAdd(&g_mxb_wait_timeouts, 1u);
-  return false;
-}
 
 template <bool kGlu, int kT>
 __global__ void __launch_bounds__(kNarrowThreads, 1) grouped_narrow_kernel(
@@ -652,7 +743,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) grouped_narrow_kernel(
             for (int b = 0; b < kBlocks; ++b)
               tc_mma(tmem + (uint32_t)((buf * kBlocks + b) * kT),
                      smem_desc_sw128(st + b * kBoxBytes) + (uint64_t)(2 * j),
-                     dr + (uint64_t)(2 * j), mxf4_idesc(kT, sf_id),
+                     dr + (uint64_t)(2 * j), mxf4_idesc(128, kT, sf_id),
                      (sfw + 8 * b + 4 * (j >> 1)) | (sf_id << 30),
                      (sfr + 4 * (j >> 1)) | (sf_id << 30), (ks > k_begin || j > 0) ? 1u : 0u);
           }
@@ -763,27 +854,12 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) grouped_narrow_kernel(
     // ------------------------------------------------ the rows' scale bytes
     const int r = (warp - 6) * 32 + lane;
     if ((warp - 6) * 32 < kT) {
-      const int mode = scale_mode(p);
-      uint2 next[4];
-      auto fetch = [&](const Tile& tl, int ks0) {
-        const int64_t row = (int64_t)tl.m0 + r;
-        const uint8_t* src = p.a_scales + row * p.a_spitch;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          next[j] = r < kT && row < p.M && ks0 + j < k_end ? row_scales(src, S, ks0 + j, mode)
-                                                           : make_uint2(0u, 0u);
-      };
+      RowScales<decltype(tile_at)> mine(p, tile_at, r < kT ? r : -1, k_begin, k_end, my_tiles);
       int gs = 0;
       bool ok = true;
-      if (my_tiles > 0) fetch(tile_at(0), k_begin);
       for (int i = 0; ok && i < my_tiles; ++i) {
-        const Tile tl = tile_at(i);
         for (int ks0 = k_begin; ok && ks0 < k_end; ks0 += 4) {
-          uint2 now[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) now[j] = next[j];
-          if (ks0 + 4 < k_end) fetch(tl, ks0 + 4);
-          else if (i + 1 < my_tiles) fetch(tile_at(i + 1), k_begin);
+          mine.advance();
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if (ks0 + j >= k_end) break;
@@ -795,8 +871,9 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) grouped_narrow_kernel(
             }
             uint8_t* sf = smem + s * L::kStage + kBlocks * (kBoxBytes + kAtoms) + kT * 128 +
                           lane * 16 + (warp - 6) * 4;
-            *reinterpret_cast<uint32_t*>(sf) = now[j].x;
-            *reinterpret_cast<uint32_t*>(sf + 512) = now[j].y;
+            const uint2 w = mine.get(j);
+            *reinterpret_cast<uint32_t*>(sf) = w.x;
+            *reinterpret_cast<uint32_t*>(sf + 512) = w.y;
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&full[s]);
@@ -838,7 +915,7 @@ __global__ void __launch_bounds__(256) swizzle_grouped_kernel(const uint8_t* __r
 }
 
 // ---------------------------------------------------------------- host side
-// Which kernel, and how.  rows: row-tile height (128 = wide); ranks: CTAs that
+// Which kernel, and how.  rows: row-tile height (256 = wide); ranks: CTAs that
 // split K.
 struct Plan {
   int rows, ranks;
@@ -853,9 +930,9 @@ int64_t most_tiles(int64_t M, int64_t E, int rows, int64_t ntn) {
 Plan grouped_plan(const GroupedArgs& p, bool glu) {
   const int sms = sm_count();
   const int64_t ksteps = cdiv(p.K, kStepK);
-  const int64_t wide = most_tiles(p.M, p.E, 128, cdiv(p.width, glu ? 128 : 256));
-  Plan r{128, 1, wide};
-  if (p.M > 96 * (int64_t)p.E && wide >= sms) return r;
+  const int64_t wide = most_tiles(p.M, p.E, 256, cdiv(p.width, glu ? 128 : 256));
+  Plan r{256, 1, wide};
+  if (p.M > 96 * (int64_t)p.E && wide >= sms / 2) return r;
   r.rows = p.M <= 24 * (int64_t)p.E ? 16 : 64;
   r.tiles = most_tiles(p.M, p.E, r.rows, cdiv(p.width, 128));
   const int most = p.c_codes ? 4 : 8;  // a quantized block of 32 columns has one owner
@@ -863,16 +940,40 @@ Plan grouped_plan(const GroupedArgs& p, bool glu) {
   return r;
 }
 
-template <bool kGlu>
-mxb_status launch_wide(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc,
-                       const CUtensorMap& tp, const CUtensorMap& tu, const GroupedArgs& p,
-                       const Plan& plan, cudaStream_t s) {
+template <typename... Args>
+mxb_status launch_cluster(void (*kernel)(Args...), unsigned clusters, unsigned size,
+                          unsigned threads, size_t smem, cudaStream_t s,
+                          const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(clusters * size);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = size;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    set_error("grouped_gemm_mxfp4: CUDA launch failed: %s", cudaGetErrorString(e));
+    return MXB_ERR_CUDA;
+  }
+  return MXB_OK;
+}
+
+template <int kAct>
+mxb_status launch_wide(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& ts,
+                       const CUtensorMap& tc, const CUtensorMap& tp, const CUtensorMap& tu,
+                       const GroupedArgs& p, const Plan& plan, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
-  MXB_REQUIRE(grant_smem((const void*)grouped_wide_kernel<kGlu>, kWideSmem, done), MXB_ERR_CUDA,
+  MXB_REQUIRE(grant_smem((const void*)grouped_wide_kernel<kAct>, kWideSmem, done), MXB_ERR_CUDA,
               "grouped_gemm_mxfp4: cannot reserve shared memory");
-  const unsigned grid = (unsigned)std::min<int64_t>(plan.tiles, sm_count());
-  grouped_wide_kernel<kGlu><<<grid, kWideThreads, kWideSmem, s>>>(ta, tb, tc, tp, tu, p);
-  return launch_status("grouped_gemm_mxfp4");
+  return launch_cluster(grouped_wide_kernel<kAct>,
+                        (unsigned)std::min<int64_t>(plan.tiles, std::max(1, sm_count() / 2)), 2,
+                        kWideThreads, kWideSmem, s, ta, tb, ts, tc, tp, tu, p);
 }
 
 template <bool kGlu, int kT>
@@ -882,25 +983,9 @@ mxb_status launch_narrow(const CUtensorMap& ta, const CUtensorMap& tb, const Gro
   static std::atomic<uint64_t> done{0};
   MXB_REQUIRE(grant_smem((const void*)grouped_narrow_kernel<kGlu, kT>, L::kSmem, done),
               MXB_ERR_CUDA, "grouped_gemm_mxfp4: cannot reserve shared memory");
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(std::min<int64_t>(plan.tiles, std::max(1, sm_count() / plan.ranks)) *
-                                plan.ranks));
-  cfg.blockDim = dim3(kNarrowThreads);
-  cfg.dynamicSmemBytes = L::kSmem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)plan.ranks;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, grouped_narrow_kernel<kGlu, kT>, ta, tb, p);
-  if (e != cudaSuccess) {
-    (void)cudaGetLastError();
-    set_error("grouped_gemm_mxfp4: CUDA launch failed: %s", cudaGetErrorString(e));
-    return MXB_ERR_CUDA;
-  }
-  return MXB_OK;
+  const int64_t clusters = std::min<int64_t>(plan.tiles, std::max(1, sm_count() / plan.ranks));
+  return launch_cluster(grouped_narrow_kernel<kGlu, kT>, (unsigned)clusters, (unsigned)plan.ranks,
+                        kNarrowThreads, L::kSmem, s, ta, tb, p);
 }
 
 }  // namespace
@@ -989,13 +1074,14 @@ extern "C" mxb_status mxb_grouped_gemm_mxfp4(const void* a_codes, int64_t a_code
   p.c_ld = ep->c_ld;
   p.c_codes = (uint8_t*)ep->c_codes;
   p.c_scales = (uint8_t*)ep->c_scales;
+  p.a_scales_tma = 0;
   const Plan plan = grouped_plan(p, glu);
   MXB_REQUIRE(plan.tiles <= INT32_MAX, MXB_ERR_INVALID_ARGUMENT, "%s: too many tiles", what);
 
   const cudaStream_t s = to_cuda(stream);
   CUtensorMap ta, tb;
   if (!make_tensor_map_2d(&ta, a_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, M, K / 2, a_codes_pitch,
-                          128, (uint32_t)plan.rows, CU_TENSOR_MAP_SWIZZLE_128B) ||
+                          128, (uint32_t)std::min(plan.rows, 128), CU_TENSOR_MAP_SWIZZLE_128B) ||
       !make_tensor_map_2d(&tb, b_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (int64_t)E * N, K / 2,
                           K / 2, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B))
     return MXB_ERR_CUDA;
@@ -1005,6 +1091,11 @@ extern "C" mxb_status mxb_grouped_gemm_mxfp4(const void* a_codes, int64_t a_code
   if (plan.rows == 64)
     return glu ? launch_narrow<true, 64>(ta, tb, p, plan, s)
                : launch_narrow<false, 64>(ta, tb, p, plan, s);
+  CUtensorMap ts = ta;
+  p.a_scales_tma = aligned(a_scales, 16) && a_scales_pitch % 16 == 0;
+  if (p.a_scales_tma && !make_tensor_map_2d(&ts, a_scales, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, M,
+                                            K / 32, a_scales_pitch, 32, 128))
+    return MXB_ERR_CUDA;
   // output maps are one part wide, so that a box never reaches into the other part
   CUtensorMap tc = ta, tp = ta, tu = ta;
   auto out_map = [&](CUtensorMap* m, void* base, int64_t ld) {
@@ -1014,6 +1105,13 @@ extern "C" mxb_status mxb_grouped_gemm_mxfp4(const void* a_codes, int64_t a_code
   if ((c && !out_map(&tc, c, ep->c_ld)) || (ep->pre && !out_map(&tp, ep->pre, ep->pre_ld)) ||
       (ep->pre && glu && !out_map(&tu, (uint8_t*)ep->pre + W * 2, ep->pre_ld)))
     return MXB_ERR_CUDA;
-  return glu ? launch_wide<true>(ta, tb, tc, tp, tu, p, plan, s)
-             : launch_wide<false>(ta, tb, tc, tp, tu, p, plan, s);
+  switch (p.act) {
+    case MXB_ACT_RELU: return launch_wide<MXB_ACT_RELU>(ta, tb, ts, tc, tp, tu, p, plan, s);
+    case MXB_ACT_RELU2: return launch_wide<MXB_ACT_RELU2>(ta, tb, ts, tc, tp, tu, p, plan, s);
+    case MXB_ACT_SILU: return launch_wide<MXB_ACT_SILU>(ta, tb, ts, tc, tp, tu, p, plan, s);
+    case MXB_ACT_GELU: return launch_wide<MXB_ACT_GELU>(ta, tb, ts, tc, tp, tu, p, plan, s);
+    case MXB_ACT_GELU_TANH: return launch_wide<MXB_ACT_GELU_TANH>(ta, tb, ts, tc, tp, tu, p, plan, s);
+    case MXB_ACT_SWIGLU: return launch_wide<MXB_ACT_SWIGLU>(ta, tb, ts, tc, tp, tu, p, plan, s);
+    default: return launch_wide<MXB_ACT_NONE>(ta, tb, ts, tc, tp, tu, p, plan, s);
+  }
 }

@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) grouped_wgrad_kernel(
 #pragma unroll
           for (int j = 0; j < kWgRows / 16; ++j)  // 16 rows of 128 bytes further each
             tc_mma_bf16(tmem + (uint32_t)(buf * kTileY), dx + (uint64_t)(128 * j),
-                        dyd + (uint64_t)(128 * j), bf16_mn_idesc(kTileY),
+                        dyd + (uint64_t)(128 * j), bf16_mn_idesc(128, kTileY),
                         (st > 0 || j > 0) ? 1u : 0u);
           tc_commit(&empty[s]);
         }
