@@ -146,10 +146,9 @@ __device__ __forceinline__ float load_bias(const GroupedArgs& p, int64_t i) {
 //   warps 4-7    scales: each warp gathers its lane quadrant's words of a step
 //                from shared memory and writes them to the step's tensor memory
 //                columns with tcgen05.st, so that the tensor pipe carries MMAs
-//                only.  The scales have rings of their own, deeper than the
-//                codes': their path is longer (copy, shared memory, tensor
-//                memory).  Rows that TMA cannot take (a pitch that is not a
-//                multiple of 16) are read by these warps, a row a thread
+//                only, and arrives on the barrier that the codes complete on:
+//                one wait a step.  Rows that TMA cannot take (a pitch that is not
+//                a multiple of 16) are read by these warps, a row a thread
 //   warps 8-15   epilogue: two groups of four warps, each with half the columns.
 //                The accumulator is read into registers at once and given back,
 //                so that the next tile's products run under the epilogue
@@ -162,7 +161,6 @@ constexpr int kSbStages = 2;               // shared-memory scales of four steps
 constexpr uint32_t kSbA = 128 * 32;        // A's 128 rows of 32 bytes,
 constexpr uint32_t kSbB = 4 * kAtoms;      // 8 atoms of each of B's halves
 constexpr uint32_t kSbStage = kSbA + 2 * kSbB;
-constexpr int kSfStages = 8;               // steps of scales in tensor memory
 constexpr uint32_t kOutBox = 128 * 64;     // 128 rows x 32 bf16 columns, 64-byte swizzle
 constexpr int kOutSlots = 4;               // per epilogue group
 constexpr uint32_t kScaleCol = 256;        // tensor memory: accumulator, then scales
@@ -170,7 +168,7 @@ constexpr uint32_t kTmemCols = 512;
 constexpr size_t kWideSmem = 1024 + kWideStages * kWideStage + kSbStages * kSbStage +
                              2 * kOutSlots * kOutBox + 256 * 4 + kGroupTableInts * 4 + 512;
 static_assert(kWideSmem <= 227 * 1024, "one CTA per SM");
-static_assert(kScaleCol + 24 * kSfStages <= kTmemCols, "scales fit beside the accumulator");
+static_assert(kScaleCol + 24 * kWideStages <= kTmemCols, "scales fit beside the accumulator");
 static_assert(kWideStage % 1024 == 0, "swizzled boxes start on 1024 bytes");
 // Registers: 512 threads x 128 at launch = 128 x 64 + 128 x 96 + 256 x 176.  The
 // scale warps must not spill: a spilled load is waited for where it is issued.
@@ -189,13 +187,12 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
   uint8_t* scales = smem + kWideStages * kWideStage;
   uint8_t* out_boxes = scales + kSbStages * kSbStage;
   float* bias_s = reinterpret_cast<float*>(out_boxes + 2 * kOutSlots * kOutBox);
-  uint64_t* full = reinterpret_cast<uint64_t*>(bias_s + 256);  // CTA 0's: codes of both CTAs
+  // CTA 0's: a step's codes of both CTAs have landed and its scales are in tensor memory
+  uint64_t* full = reinterpret_cast<uint64_t*>(bias_s + 256);
   uint64_t* empty = full + kWideStages;
   uint64_t* sb_full = empty + kWideStages;   // four steps' scales in shared memory
   uint64_t* sb_empty = sb_full + kSbStages;
-  uint64_t* sf_full = sb_empty + kSbStages;  // CTA 0's: a step's scales in tensor memory
-  uint64_t* sf_empty = sf_full + kSfStages;
-  uint64_t* acc_full = sf_empty + kSfStages;
+  uint64_t* acc_full = sb_empty + kSbStages;
   uint64_t* acc_empty = acc_full + 1;  // CTA 0's
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 1);
   int* failed = reinterpret_cast<int*>(tmem_slot + 1);
@@ -215,16 +212,12 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
     tmem_alloc_pair(tmem_slot, kTmemCols);
   } else if (t == 64) {
     for (int s = 0; s < kWideStages; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], 1 + 8);
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < kSbStages; ++s) {
       mbar_init(&sb_full[s], 1);
       mbar_init(&sb_empty[s], 4);
-    }
-    for (int s = 0; s < kSfStages; ++s) {
-      mbar_init(&sf_full[s], 8);
-      mbar_init(&sf_empty[s], 1);
     }
     mbar_init(acc_full, 1);
     mbar_init(acc_empty, 16);
@@ -317,7 +310,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
     } else if (warp == 1 && rank == 0) {
       // ------------------------------------------------ MMA issuer
       const bool one = elect_one();
-      bool ok = true;
+      bool ok = true, ready = false;
       int gs = 0;
       for (int i = 0; ok && i < my_tiles; ++i) {
         if (i > 0 && !mbar_wait(acc_empty, (uint32_t)((i - 1) & 1))) {
@@ -326,16 +319,17 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
         }
         tc_fence_after();
         for (int ks = 0; ks < ksteps; ++ks, ++gs) {
-          const int s = gs % kWideStages, f = gs % kSfStages;
-          if (!mbar_wait(&sf_full[f], (uint32_t)((gs / kSfStages) & 1)) ||
-              !mbar_wait(&full[s], (uint32_t)((gs / kWideStages) & 1))) {
+          const int s = gs % kWideStages;
+          if (!ready && !mbar_wait(&full[s], (uint32_t)((gs / kWideStages) & 1))) {
             ok = false;
             break;
           }
+          // whether the next step is ready as well: known by the time it is needed
+          ready = mbar_peek(&full[(gs + 1) % kWideStages], (uint32_t)(((gs + 1) / kWideStages) & 1));
           tc_fence_after();
           __syncwarp();
           const uint8_t* st = smem + s * kWideStage;
-          const uint32_t sfc = tmem + kScaleCol + (uint32_t)(f * 24);
+          const uint32_t sfc = tmem + kScaleCol + (uint32_t)(s * 24);
           const int left = p.K - ks * kStepK;  // elements of K from this step on
           const uint64_t da = smem_desc_sw128(st);
           const uint64_t db = smem_desc_sw128(st + kBoxBytes);
@@ -348,7 +342,6 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
                         (sfc + 8 + 8 * (j >> 1)) | (sf_id << 30), (ks > 0 || j > 0) ? 1u : 0u, one);
           }
           tc_commit_pair(&empty[s], one);
-          tc_commit_pair(&sf_empty[f], one);
         }
         __syncwarp();
         tc_commit_pair(acc_full, one);
@@ -359,7 +352,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideScaleRegs));
     // ------------------------------------------------ scales
     const int q = warp - 4, r = q * 32 + lane;
-    const uint32_t sf_full0 = peer_addr(smem_addr(sf_full), 0);
+    const uint32_t full0 = peer_addr(smem_addr(full), 0);
     const uint32_t col0 = tmem + ((uint32_t)(q * 32) << 16) + kScaleCol;
     RowScales<decltype(tile_at)> rows(p, tile_at, r, 0, ksteps, p.a_scales_tma ? 0 : my_tiles);
     int gs = 0, gq = 0;
@@ -401,9 +394,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
                   sb + kSbA + (k & 1) * kSbB + (2 * (j + h) + (k >> 1)) * 512 + lane * 16);
               b[4 * k] = w.x; b[4 * k + 1] = w.y; b[4 * k + 2] = w.z; b[4 * k + 3] = w.w;
             }
-            const int s = gs % kSfStages;
-            up = up && (gs < kSfStages ||
-                        mbar_wait(&sf_empty[s], (uint32_t)((gs / kSfStages - 1) & 1)));
+            const int s = gs % kWideStages;
+            up = up && (gs < kWideStages ||
+                        mbar_wait(&empty[s], (uint32_t)((gs / kWideStages - 1) & 1)));
             tc_fence_after();
             __syncwarp();
             tmem_st8(col0 + (uint32_t)(s * 24), a);
@@ -411,7 +404,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) peer_signal(sf_full0 + 8 * s);
+            if (lane == 0) peer_signal(full0 + 8 * s);
             ++gs;
           }
         }

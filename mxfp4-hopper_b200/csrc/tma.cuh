@@ -87,6 +87,20 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
   return false;
 }
 
+// Whether that phase has completed, without waiting; the answer may be used
+// later, so that its latency passes under other work.
+__device__ __forceinline__ bool mbar_peek(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n"
+      " mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+
 // 2-D tiled TMA load of box {x .. x+bx, y .. y+by} into shared memory,
 // completion signalled on `bar` (complete_tx).  x * element size must be a
 // multiple of 16 bytes; out-of-range elements are filled with zero.
