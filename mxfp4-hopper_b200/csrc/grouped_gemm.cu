@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
         const bool second = has_second(tl);
         for (int ks = 0; ks < ksteps; ++ks, ++gs) {
           const int s = gs % kWideStages;
-          if (gs >= kWideStages && !mbar_wait(&empty[s], (uint32_t)((gs / kWideStages - 1) & 1))) {
+          if (gs >= kWideStages && !mbar_wait_suspend(&empty[s], (uint32_t)((gs / kWideStages - 1) & 1))) {
             atomicExch(failed, 1);
             ok = false;
             break;
@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
       }
       // do not leave while copies are still landing (CTA 0 waits for both CTAs' codes)
       for (int q = gs > kWideStages ? gs - kWideStages : 0; rank == 0 && q < gs; ++q)
-        mbar_wait(&full[q % kWideStages], (uint32_t)((q / kWideStages) & 1));
+        mbar_wait_suspend(&full[q % kWideStages], (uint32_t)((q / kWideStages) & 1));
     } else if (warp == 2 && lane == 0) {
       // ------------------------------------------------ scales, four steps a time
       const int nbp = (p.width + 127) / 128;  // 128-row scale blocks of a weight part
@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
         const bool second = has_second(tl);
         for (int k4 = 0; k4 < S4; k4 += 8, ++gq) {
           const int s = gq % kSbStages;
-          if (gq >= kSbStages && !mbar_wait(&sb_empty[s], (uint32_t)((gq / kSbStages - 1) & 1))) {
+          if (gq >= kSbStages && !mbar_wait_suspend(&sb_empty[s], (uint32_t)((gq / kSbStages - 1) & 1))) {
             atomicExch(failed, 1);
             ok = false;
             break;
@@ -306,21 +306,21 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
         }
       }
       for (int q = gq > kSbStages ? gq - kSbStages : 0; q < gq; ++q)
-        mbar_wait(&sb_full[q % kSbStages], (uint32_t)((q / kSbStages) & 1));
+        mbar_wait_suspend(&sb_full[q % kSbStages], (uint32_t)((q / kSbStages) & 1));
     } else if (warp == 1 && rank == 0) {
       // ------------------------------------------------ MMA issuer
       const bool one = elect_one();
       bool ok = true, ready = false;
       int gs = 0;
       for (int i = 0; ok && i < my_tiles; ++i) {
-        if (i > 0 && !mbar_wait(acc_empty, (uint32_t)((i - 1) & 1))) {
+        if (i > 0 && !mbar_wait_suspend(acc_empty, (uint32_t)((i - 1) & 1))) {
           ok = false;
           break;
         }
         tc_fence_after();
         for (int ks = 0; ks < ksteps; ++ks, ++gs) {
           const int s = gs % kWideStages;
-          if (!ready && !mbar_wait(&full[s], (uint32_t)((gs / kWideStages) & 1))) {
+          if (!ready && !mbar_wait_suspend(&full[s], (uint32_t)((gs / kWideStages) & 1))) {
             ok = false;
             break;
           }
@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
       for (int ks0 = 0; ok && ks0 < ksteps; ks0 += 4, ++gq) {
         const int sq = gq % kSbStages;
         uint8_t* sb = scales + sq * kSbStage;
-        bool up = mbar_wait(&sb_full[sq], (uint32_t)((gq / kSbStages) & 1));
+        bool up = mbar_wait_suspend(&sb_full[sq], (uint32_t)((gq / kSbStages) & 1));
         if (!p.a_scales_tma) {
           rows.advance();
 #pragma unroll
@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
             }
             const int s = gs % kWideStages;
             up = up && (gs < kWideStages ||
-                        mbar_wait(&empty[s], (uint32_t)((gs / kWideStages - 1) & 1)));
+                        mbar_wait_suspend(&empty[s], (uint32_t)((gs / kWideStages - 1) & 1)));
             tc_fence_after();
             __syncwarp();
             tmem_st8(col0 + (uint32_t)(s * 24), a);
@@ -444,7 +444,21 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
         if (col < p.width) bias = load_bias(p, at);
       }
       bias_h[ht] = bias;
-      const bool ok = mbar_wait(acc_full, (uint32_t)(i & 1));
+      const bool whole = rows == 128;
+      const int64_t row = (int64_t)tl.m0 + r;
+      // this row's residual of one chunk of 32 columns, read a chunk ahead
+      uint4 res[4];
+      auto load_residual = [&](int n) {
+        const uint8_t* src = p.residual + (row * p.residual_ld + n) * 2;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          res[k] = make_uint4(0u, 0u, 0u, 0u);
+          if (p.residual && r < rows && n + 8 * k < p.width)
+            res[k] = __ldg(reinterpret_cast<const uint4*>(src + 16 * k));
+        }
+      };
+      load_residual(nh);
+      const bool ok = mbar_wait_suspend(acc_full, (uint32_t)(i & 1));
       tc_fence_after();
       const bool live = ok && !*((volatile int*)failed);
       if (named_sync_or(1 + half, 128, !live)) break;  // the four warps leave together
@@ -460,28 +474,33 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
       __syncwarp();
       if (lane == 0) peer_signal(acc_empty0);
       if (rows <= 0) continue;
-      const bool whole = rows == 128;
-      const int64_t row = (int64_t)tl.m0 + r;
-#pragma unroll
+      // One copy of the code for all chunks (unrolled four times it runs from beyond
+      // the instruction caches, at half the rate): the registers move down instead.
+#pragma unroll 1
       for (int ch = 0; ch < kHalfN / 32; ++ch) {
         const int n = nh + 32 * ch;
-        if (n < p.width) {
-          uint4 res[4];
-          if (p.residual) {
-            const uint8_t* src = p.residual + (row * p.residual_ld + n) * 2;
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              res[k] = r < rows && n + 8 * k < p.width
-                           ? *reinterpret_cast<const uint4*>(src + 16 * k)
-                           : make_uint4(0u, 0u, 0u, 0u);
-          }
+        if (n >= p.width) break;
+        {
           float v[32], u[kGlu ? 32 : 1];
+          auto add_bias = [&](const uint32_t* a, const float* b, float* z) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(acc[32 * ch + j]) + bias_h[32 * ch + j];
+            for (int j = 0; j < 32; j += 4) {
+              const float4 w = *reinterpret_cast<const float4*>(b + j);
+              add2(F2(__uint_as_float(a[j]), __uint_as_float(a[j + 1])), F2(w.x, w.y)).get(z[j], z[j + 1]);
+              add2(F2(__uint_as_float(a[j + 2]), __uint_as_float(a[j + 3])), F2(w.z, w.w)).get(z[j + 2], z[j + 3]);
+            }
+          };
+          add_bias(acc, bias_h + 32 * ch, v);
+          if constexpr (kGlu) add_bias(acc + 64, bias_h + 64 + 32 * ch, u);
           if constexpr (kGlu) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              u[j] = __uint_as_float(acc[64 + 32 * ch + j]) + bias_h[64 + 32 * ch + j];
+            for (int j = 0; j < 32; ++j) {
+              acc[j] = acc[32 + j];
+              acc[64 + j] = acc[96 + j];
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 96; ++j) acc[j] = acc[32 + j];
           }
           // the boxes of this set have been read by the stores issued `sets` chunks ago
           if (issuer) {
@@ -502,14 +521,17 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
             if constexpr (kGlu) put(bx + kOutBox, u);
           }
           if constexpr (kGlu) {
+            act_each<MXB_ACT_SILU>(v);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = act_value<MXB_ACT_SILU>(v[j]) * u[j];
+            for (int j = 0; j < 32; j += 2)
+              mul2(F2(v[j], v[j + 1]), F2(u[j], u[j + 1])).get(v[j], v[j + 1]);
           } else {
             act_each<kAct>(v);
           }
           if (p.residual) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) add8_bf16(v + 8 * k, res[k]);
+            if (32 * (ch + 1) < kHalfN) load_residual(n + 32);
           }
           if (p.c) put(bx + n_pre * kOutBox, v);
           if (p.c_codes && r < rows) {

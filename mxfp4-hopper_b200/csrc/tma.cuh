@@ -87,6 +87,27 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
   return false;
 }
 
+// mbar_wait() that lets the hardware suspend the thread for up to kSuspendNs a
+// round instead of polling, so that waiting warps leave the issue slots to the
+// others.  kSuspendRounds bound the wait at a second or so.
+constexpr uint32_t kSuspendNs = 10000, kSuspendRounds = 1u << 17;
+__device__ __forceinline__ bool mbar_wait_suspend(uint64_t* bar, uint32_t parity) {
+  const uint32_t a = smem_addr(bar);
+  for (uint32_t i = 0; i < kSuspendRounds; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n"
+        " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+        " selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(a), "r"(parity), "r"(kSuspendNs)
+        : "memory");
+    if (done) return true;
+  }
+  atomicAdd(&g_mxb_wait_timeouts, 1u);
+  return false;
+}
+
 // Whether that phase has completed, without waiting; the answer may be used
 // later, so that its latency passes under other work.
 __device__ __forceinline__ bool mbar_peek(uint64_t* bar, uint32_t parity) {
