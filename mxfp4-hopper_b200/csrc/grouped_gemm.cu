@@ -955,30 +955,6 @@ Plan grouped_plan(const GroupedArgs& p, bool glu) {
   return r;
 }
 
-template <typename... Args>
-mxb_status launch_cluster(void (*kernel)(Args...), unsigned clusters, unsigned size,
-                          unsigned threads, size_t smem, cudaStream_t s,
-                          const Args&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(clusters * size);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = size;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
-  if (e != cudaSuccess) {
-    (void)cudaGetLastError();
-    set_error("grouped_gemm_mxfp4: CUDA launch failed: %s", cudaGetErrorString(e));
-    return MXB_ERR_CUDA;
-  }
-  return MXB_OK;
-}
-
 template <int kAct>
 mxb_status launch_wide(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& ts,
                        const CUtensorMap& tc, const CUtensorMap& tp, const CUtensorMap& tu,
@@ -986,7 +962,7 @@ mxb_status launch_wide(const CUtensorMap& ta, const CUtensorMap& tb, const CUten
   static std::atomic<uint64_t> done{0};
   MXB_REQUIRE(grant_smem((const void*)grouped_wide_kernel<kAct>, kWideSmem, done), MXB_ERR_CUDA,
               "grouped_gemm_mxfp4: cannot reserve shared memory");
-  return launch_cluster(grouped_wide_kernel<kAct>,
+  return launch_cluster("grouped_gemm_mxfp4", grouped_wide_kernel<kAct>,
                         (unsigned)std::min<int64_t>(plan.tiles, std::max(1, sm_count() / 2)), 2,
                         kWideThreads, kWideSmem, s, ta, tb, ts, tc, tp, tu, p);
 }
@@ -999,7 +975,7 @@ mxb_status launch_narrow(const CUtensorMap& ta, const CUtensorMap& tb, const Gro
   MXB_REQUIRE(grant_smem((const void*)grouped_narrow_kernel<kGlu, kT>, L::kSmem, done),
               MXB_ERR_CUDA, "grouped_gemm_mxfp4: cannot reserve shared memory");
   const int64_t clusters = std::min<int64_t>(plan.tiles, std::max(1, sm_count() / plan.ranks));
-  return launch_cluster(grouped_narrow_kernel<kGlu, kT>, (unsigned)clusters, (unsigned)plan.ranks,
+  return launch_cluster("grouped_gemm_mxfp4", grouped_narrow_kernel<kGlu, kT>, (unsigned)clusters, (unsigned)plan.ranks,
                         kNarrowThreads, L::kSmem, s, ta, tb, p);
 }
 

@@ -6,9 +6,10 @@
 // are MN-major for the tensor core and neither is transposed in memory.  An
 // E2M1 value times 2^(e - 127) is exact in BF16: eight warps expand x's codes
 // into a BF16 tile in shared memory while the tensor core works on the tiles
-// before, and the product is kind::f16 (BF16 x BF16 -> f32).  The tile is 128
-// columns of x (the M side: half the expanding work of 256) by 256 columns of
-// dy, 64 rows a step.
+// before, and the product is kind::f16 (BF16 x BF16 -> f32).  Two CTAs share a
+// tile (cta_group::2) of 256 columns of x, the M side, 128 expanded by each, by
+// 256 columns of dy, 128 loaded by each, 64 rows a step: every byte of dy and x
+// crosses L2 -> shared memory once per 256 columns of the other.
 //
 // Ragged groups: a step's rows past its expert's end are expanded as zeros, and
 // the same rows of dy (the next expert's, whatever they hold) are overwritten
@@ -29,11 +30,11 @@ namespace mxb {
 namespace {
 
 constexpr int kWgThreads = 448;  // TMA, MMA, 4 epilogue warps, 8 expanding warps
-constexpr int kWgStages = 4;
-constexpr int kWgRows = 64;                      // rows per step
-constexpr int kTileX = 128, kTileY = 256;        // columns of x and of dy
-constexpr uint32_t kWgBox = kWgRows * 128;       // 64 rows x 64 bf16 columns
-constexpr uint32_t kWgStage = (kTileX + kTileY) / 64 * kWgBox;
+constexpr int kWgStages = 6;
+constexpr int kWgRows = 64;                 // rows per step
+constexpr int kTileX = 256, kTileY = 256;   // columns of x and of dy, half in each CTA
+constexpr uint32_t kWgBox = kWgRows * 128;  // 64 rows x 64 bf16 columns
+constexpr uint32_t kWgX = 2 * kWgBox, kWgStage = 2 * kWgX;
 constexpr size_t kWgSmem = 1024 + kWgStages * kWgStage + kGroupTableInts * 4 + 256;
 static_assert(kWgSmem <= 227 * 1024, "one CTA per SM");
 
@@ -79,10 +80,10 @@ __global__ void __launch_bounds__(kWgThreads, 1) grouped_wgrad_kernel(
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
   uint64_t* dy_full = reinterpret_cast<uint64_t*>(smem + kWgStages * kWgStage);
-  uint64_t* x_full = dy_full + kWgStages;
-  uint64_t* empty = x_full + kWgStages;
+  uint64_t* full = dy_full + kWgStages;  // CTA 0's: both CTAs' halves are in place
+  uint64_t* empty = full + kWgStages;
   uint64_t* acc_full = empty + kWgStages;  // [2]
-  uint64_t* acc_empty = acc_full + 2;      // [2]
+  uint64_t* acc_empty = acc_full + 2;      // [2], CTA 0's
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   int* failed = reinterpret_cast<int*>(tmem_slot + 1);
   GroupTable g;
@@ -91,21 +92,21 @@ __global__ void __launch_bounds__(kWgThreads, 1) grouped_wgrad_kernel(
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const int nty = (p.N + kTileY - 1) / kTileY, ntx = (p.K + kTileX - 1) / kTileX;
   const int per_expert = nty * ntx;
+  const int rank = (int)cluster_rank();
 
   if (warp == 0) {
     build_groups(g, p.m_splits, p.E, p.M, [&](int) { return 0; });
   } else if (warp == 1) {
-    tmem_alloc(tmem_slot, 512);
-    tmem_relinquish();
+    tmem_alloc_pair(tmem_slot, 512);
   } else if (t == 64) {
     for (int s = 0; s < kWgStages; ++s) {
       mbar_init(&dy_full[s], 1);
-      mbar_init(&x_full[s], 8);
+      mbar_init(&full[s], 16);
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 4);
+      mbar_init(&acc_empty[b], 8);
     }
     fence_mbar_init();
     *failed = 0;
@@ -113,20 +114,21 @@ __global__ void __launch_bounds__(kWgThreads, 1) grouped_wgrad_kernel(
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  cluster_sync();
   const uint32_t tmem = *tmem_slot;
   const int tiles = p.E * per_expert;
-  const int my_tiles =
-      (int)blockIdx.x < tiles ? (tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+  const int pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;
+  const int my_tiles = pair < tiles ? (tiles - 1 - pair) / pairs + 1 : 0;
 
   struct Tile {
-    int e, x0, y0, row0, rows, steps;
+    int e, x0, y0, row0, rows, steps;  // x0: this CTA's columns of x; y0: the pair's of dy
   };
   auto tile_at = [&](int i) {
-    const int id = (int)blockIdx.x + i * (int)gridDim.x;
+    const int id = pair + i * pairs;
     Tile r;
     r.e = id / per_expert;
     const int local = id % per_expert;
-    r.x0 = local / nty * kTileX;
+    r.x0 = local / nty * kTileX + rank * (kTileX / 2);
     r.y0 = local % nty * kTileY;
     r.row0 = g.off[r.e];
     r.rows = g.off[r.e + 1] - r.row0;
@@ -143,65 +145,69 @@ __global__ void __launch_bounds__(kWgThreads, 1) grouped_wgrad_kernel(
         const Tile tl = tile_at(i);
         for (int st = 0; st < tl.steps; ++st) {
           const int s = gs % kWgStages;
-          if (gs >= kWgStages && !mbar_wait(&empty[s], (uint32_t)((gs / kWgStages - 1) & 1))) {
+          if (gs >= kWgStages && !mbar_wait_suspend(&empty[s], (uint32_t)((gs / kWgStages - 1) & 1))) {
             atomicExch(failed, 1);
             ok = false;
             break;
           }
-          uint8_t* dst = smem + s * kWgStage + kTileX / 64 * kWgBox;
-          const int boxes = min(kTileY / 64, (p.N - tl.y0 + 63) / 64);
-          mbar_arrive_expect_tx(&dy_full[s], (uint32_t)boxes * kWgBox);
-          for (int b = 0; b < boxes; ++b)
-            tma_load_2d(dst + b * kWgBox, &map_dy, tl.y0 + 64 * b, tl.row0 + st * kWgRows,
-                        &dy_full[s]);
+          // both boxes, also past dy's last column (zeros): the wait has one form
+          mbar_arrive_expect_tx(&dy_full[s], 2 * kWgBox);
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+            tma_load_2d(smem + s * kWgStage + kWgX + b * kWgBox, &map_dy,
+                        tl.y0 + rank * (kTileY / 2) + 64 * b, tl.row0 + st * kWgRows, &dy_full[s]);
           ++gs;
         }
       }
       // do not leave while copies of this CTA are still landing
       for (int q = gs > kWgStages ? gs - kWgStages : 0; q < gs; ++q)
-        mbar_wait(&dy_full[q % kWgStages], (uint32_t)((q / kWgStages) & 1));
+        mbar_wait_suspend(&dy_full[q % kWgStages], (uint32_t)((q / kWgStages) & 1));
     }
   } else if (warp == 1) {
     // ------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      bool ok = true;
+    if (rank == 0) {
+      const bool one = elect_one();
+      bool ok = true, ready = false;
       int gs = 0;
       for (int i = 0; ok && i < my_tiles; ++i) {
         const int buf = i & 1, steps = tile_at(i).steps;
-        if (i > 1 && !mbar_wait(&acc_empty[buf], (uint32_t)((i / 2 - 1) & 1))) {
+        if (i > 1 && !mbar_wait_suspend(&acc_empty[buf], (uint32_t)((i / 2 - 1) & 1))) {
           ok = false;
           break;
         }
         tc_fence_after();
         for (int st = 0; st < steps; ++st, ++gs) {
           const int s = gs % kWgStages;
-          const uint32_t ph = (uint32_t)((gs / kWgStages) & 1);
-          if (!mbar_wait(&dy_full[s], ph) || !mbar_wait(&x_full[s], ph)) {
+          if (!ready && !mbar_wait_suspend(&full[s], (uint32_t)((gs / kWgStages) & 1))) {
             ok = false;
             break;
           }
+          // whether the next step is ready as well: known by the time it is needed
+          ready = mbar_peek(&full[(gs + 1) % kWgStages], (uint32_t)(((gs + 1) / kWgStages) & 1));
           tc_fence_after();
+          __syncwarp();
           const uint64_t dx = smem_desc_mn_sw128(smem + s * kWgStage, kWgBox);
-          const uint64_t dyd =
-              smem_desc_mn_sw128(smem + s * kWgStage + kTileX / 64 * kWgBox, kWgBox);
+          const uint64_t dyd = smem_desc_mn_sw128(smem + s * kWgStage + kWgX, kWgBox);
 #pragma unroll
           for (int j = 0; j < kWgRows / 16; ++j)  // 16 rows of 128 bytes further each
-            tc_mma_bf16(tmem + (uint32_t)(buf * kTileY), dx + (uint64_t)(128 * j),
-                        dyd + (uint64_t)(128 * j), bf16_mn_idesc(128, kTileY),
-                        (st > 0 || j > 0) ? 1u : 0u);
-          tc_commit(&empty[s]);
+            tc_mma_bf16_pair(tmem + (uint32_t)(buf * kTileY), dx + (uint64_t)(128 * j),
+                             dyd + (uint64_t)(128 * j), bf16_mn_idesc(kTileX, kTileY),
+                             (st > 0 || j > 0) ? 1u : 0u, one);
+          tc_commit_pair(&empty[s], one);
         }
-        tc_commit(&acc_full[buf]);
+        __syncwarp();
+        tc_commit_pair(&acc_full[buf], one);
       }
       if (!ok) atomicExch(failed, 1);
     }
   } else if (warp < 6) {
     // ------------------------------------------------ epilogue: lane = column of x
     const int quad = warp & 3;
+    const uint32_t acc_empty0 = peer_addr(smem_addr(acc_empty), 0);
     for (int i = 0; i < my_tiles; ++i) {
       const Tile tl = tile_at(i);
       const int buf = i & 1;
-      const bool ok = mbar_wait(&acc_full[buf], (uint32_t)((i / 2) & 1));
+      const bool ok = mbar_wait_suspend(&acc_full[buf], (uint32_t)((i / 2) & 1));
       tc_fence_after();
       if (named_sync_or(1, 128, !ok || *((volatile int*)failed))) break;
       const int k = tl.x0 + quad * 32 + lane;
@@ -250,7 +256,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) grouped_wgrad_kernel(
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[buf]);
+      if (lane == 0) peer_signal(acc_empty0 + 8 * buf);
     }
   } else {
     // ------------------------------------------------ x: MXFP4 -> BF16 tile
@@ -260,6 +266,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) grouped_wgrad_kernel(
     // distinct.  The codes of the next kAhead steps are in registers.
     constexpr int kAhead = 4;
     const int c = warp - 6, b = lane >> 3, r = c * 8 + (lane & 7);
+    const uint32_t full0 = peer_addr(smem_addr(full), 0);
     uint4 codes[kAhead];
     uint32_t scale[kAhead];
     int li = 0, lst = 0;  // tile and step of the next load
@@ -306,7 +313,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) grouped_wgrad_kernel(
       for (int j = 0; j < kAhead; ++j) {
         if (i >= my_tiles) break;
         const int s = gs % kWgStages;
-        if (gs >= kWgStages && !mbar_wait(&empty[s], (uint32_t)((gs / kWgStages - 1) & 1))) {
+        if (gs >= kWgStages && !mbar_wait_suspend(&empty[s], (uint32_t)((gs / kWgStages - 1) & 1))) {
           atomicExch(failed, 1);
           ok = false;
           break;
@@ -319,23 +326,21 @@ __global__ void __launch_bounds__(kWgThreads, 1) grouped_wgrad_kernel(
           *reinterpret_cast<uint4*>(box + ((((b & 1) * 4 + q) ^ (r & 7)) << 4)) =
               make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
         load(codes[j], scale[j]);
+        if (!mbar_wait_suspend(&dy_full[s], (uint32_t)((gs / kWgStages) & 1))) {
+          atomicExch(failed, 1);
+          ok = false;
+          break;
+        }
         const int here = tl.rows - st * kWgRows;  // rows of the expert in this step
-        if (here < kWgRows) {
-          if (!mbar_wait(&dy_full[s], (uint32_t)((gs / kWgStages) & 1))) {
-            atomicExch(failed, 1);
-            ok = false;
-            break;
-          }
-          if (r >= here) {  // a row's four lanes: one box of 64 columns each
-            uint8_t* dyr = smem + s * kWgStage + (kTileX / 64 + b) * kWgBox + r * 128;
+        if (r >= here) {  // past its last: a row's four lanes clear its four half rows of dy
+          uint8_t* dyr = smem + s * kWgStage + kWgX + (b >> 1) * kWgBox + r * 128 + (b & 1) * 64;
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
-              *reinterpret_cast<uint4*>(dyr + 16 * q) = make_uint4(0u, 0u, 0u, 0u);
-          }
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<uint4*>(dyr + 16 * q) = make_uint4(0u, 0u, 0u, 0u);
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&x_full[s]);
+        if (lane == 0) peer_signal(full0 + 8 * s);
         ++gs;
         if (++st == tl.steps) {
           st = 0;
@@ -347,7 +352,10 @@ __global__ void __launch_bounds__(kWgThreads, 1) grouped_wgrad_kernel(
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, 512);
+  cluster_sync();  // both CTAs' products and copies have completed
+  if (warp == 1) tmem_dealloc_pair(tmem, 512);
+  __syncwarp();
+  cluster_sync();
 }
 
 template <bool kF32>
@@ -357,9 +365,9 @@ mxb_status launch_wgrad(const CUtensorMap& map, const WgradArgs& p, cudaStream_t
               "grouped_wgrad_mxfp4: cannot reserve shared memory");
   const int64_t tiles = (int64_t)p.E * cdiv(p.N, kTileY) * cdiv(p.K, kTileX);
   MXB_REQUIRE(tiles <= INT32_MAX, MXB_ERR_INVALID_ARGUMENT, "grouped_wgrad_mxfp4: too many tiles");
-  const unsigned grid = (unsigned)std::min<int64_t>(tiles, sm_count());
-  grouped_wgrad_kernel<kF32><<<grid, kWgThreads, kWgSmem, s>>>(map, p);
-  return launch_status("grouped_wgrad_mxfp4");
+  return launch_cluster("grouped_wgrad_mxfp4", grouped_wgrad_kernel<kF32>,
+                        (unsigned)std::min<int64_t>(tiles, std::max(1, sm_count() / 2)), 2,
+                        kWgThreads, kWgSmem, s, map, p);
 }
 
 }  // namespace

@@ -5,6 +5,7 @@
 #include <atomic>
 #include <cstdint>
 
+#include "capi_util.h"
 #include "common.cuh"
 
 namespace mxb {
@@ -33,6 +34,31 @@ inline int sm_count() {
     cached.store(n, std::memory_order_relaxed);
   }
   return n;
+}
+
+// Launches `clusters` clusters of `size` CTAs.
+template <typename... Args>
+mxb_status launch_cluster(const char* what, void (*kernel)(Args...), unsigned clusters, unsigned size,
+                          unsigned threads, size_t smem, cudaStream_t s,
+                          const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(clusters * size);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = size;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    set_error("%s: CUDA launch failed: %s", what, cudaGetErrorString(e));
+    return MXB_ERR_CUDA;
+  }
+  return MXB_OK;
 }
 
 }  // namespace mxb
