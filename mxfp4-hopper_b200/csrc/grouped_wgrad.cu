@@ -50,27 +50,37 @@ struct WgradArgs {
   int accumulate;
 };
 
-// 32 codes (16 bytes) and their E8M0 byte -> 32 BF16 values in element order:
-// e2m1 * 2^(e - 127) with one BF16 multiply by the power of two, whose BF16
-// pattern is e << 7 (exact; past BF16's range the product is infinite).  2^-127
-// has no normal pattern: e = 0 halves first and scales by 2^-126, also exact,
-// the result being a subnormal BF16.  e = 255 is the E8M0 NaN.
+// 32 codes (16 bytes) and their E8M0 byte -> 32 BF16 values in element order.
+// The eight magnitudes times 2^(e - 127) are made first (exact: a BF16 multiply by
+// the power of two, whose pattern is e << 7; past BF16's range they are infinite;
+// e = 0 halves first and scales by 2^-126, as 2^-127 has no normal pattern; e = 255
+// is the E8M0 NaN) and split into tables of low and high bytes, which prmt looks up
+// for four codes at a time.
 __device__ __forceinline__ void expand32(uint4 codes, uint32_t e, uint32_t (&out)[16]) {
-  const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    e2m1x4_to_bf16x4(w[i], out[4 * i], out[4 * i + 1]);
-    e2m1x4_to_bf16x4(w[i] >> 16, out[4 * i + 2], out[4 * i + 3]);
-  }
+  uint32_t m[4] = {0x3F000000u, 0x3FC03F80u, 0x40404000u, 0x40C04080u};  // 0 .5 | 1 1.5 | 2 3 | 4 6
   uint32_t f = e == 255u ? 0x7FFFu : e << 7;
-  if (e == 0u) {  // 2^-127 = 2^-126 * 1/2: halve first (exact), then scale by 2^-126
+  if (e == 0u) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) out[i] = mul_bf16x2(out[i], 0x3F003F00u);
+    for (int i = 0; i < 4; ++i) m[i] = mul_bf16x2(m[i], 0x3F003F00u);
     f = 1u << 7;
   }
   f |= f << 16;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) out[i] = mul_bf16x2(out[i], f);
+  for (int i = 0; i < 4; ++i) m[i] = mul_bf16x2(m[i], f);
+  const uint32_t lo0 = prmt(m[0], m[1], 0x6420u), lo1 = prmt(m[2], m[3], 0x6420u);
+  const uint32_t hi0 = prmt(m[0], m[1], 0x7531u), hi1 = prmt(m[2], m[3], 0x7531u);
+  const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t mag = w[i] & 0x77777777u, neg = (w[i] >> 3) & 0x11111111u;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t lo = prmt(lo0, lo1, mag >> (16 * h));
+      const uint32_t hi = prmt(hi0, hi1, mag >> (16 * h)) | prmt(0x00008000u, 0u, neg >> (16 * h));
+      out[4 * i + 2 * h] = prmt(lo, hi, 0x5140u);
+      out[4 * i + 2 * h + 1] = prmt(lo, hi, 0x7362u);
+    }
+  }
 }
 
 template <bool kF32>
@@ -101,7 +111,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) grouped_wgrad_kernel(
   } else if (t == 64) {
     for (int s = 0; s < kWgStages; ++s) {
       mbar_init(&dy_full[s], 1);
-      mbar_init(&full[s], 16);
+      mbar_init(&full[s], 4);  // a pair of warps in each CTA
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -260,94 +270,86 @@ __global__ void __launch_bounds__(kWgThreads, 1) grouped_wgrad_kernel(
     }
   } else {
     // ------------------------------------------------ x: MXFP4 -> BF16 tile
-    // Warp c has rows 8c .. 8c + 7 of a step, lane (b, r) the block of 32
-    // columns b of row r: 64 contiguous code bytes a row, and eight lanes of a
-    // 16-byte store phase in eight different rows, whose swizzled chunks are
-    // distinct.  The codes of the next kAhead steps are in registers.
-    constexpr int kAhead = 4;
-    const int c = warp - 6, b = lane >> 3, r = c * 8 + (lane & 7);
+    // Four pairs of warps take every fourth step each: expanding one is a chain of
+    // about a thousand cycles (wait, decode, shared memory, proxy fence, signal), which
+    // bound the kernel when all eight warps worked on the same step.  Warp w of a pair
+    // has rows 32w .. 32w + 31; lane (b, r) the block of 32 columns b of rows r, r + 8,
+    // ...: 64 contiguous code bytes a row, and eight lanes of a 16-byte store phase in
+    // eight different rows, whose swizzled chunks are distinct.  The codes of the
+    // pair's next step are in flight in registers.
+    const int first = (warp - 6) >> 1, b = lane >> 3;
+    const int r0 = ((warp - 6) & 1) * 32 + (lane & 7);
     const uint32_t full0 = peer_addr(smem_addr(full), 0);
-    uint4 codes[kAhead];
-    uint32_t scale[kAhead];
-    int li = 0, lst = 0;  // tile and step of the next load
-    Tile lt = {};
-    auto skip_empty = [&] {
-      while (li < my_tiles) {
-        lt = tile_at(li);
-        if (lt.steps > 0) break;
-        ++li;
-      }
+    struct At {
+      int i, st;  // tile, step in it
+      Tile tl;
     };
-    auto load = [&](uint4& q, uint32_t& e) {
-      q = make_uint4(0u, 0u, 0u, 0u);
-      e = 127u;
-      if (li >= my_tiles) return;
-      const int in = lst * kWgRows + r, k = lt.x0 + 32 * b;
-      if (in < lt.rows && k < p.K) {
-        const int64_t row = (int64_t)lt.row0 + in;
-        q = __ldg(reinterpret_cast<const uint4*>(p.x_codes + row * p.x_pitch + k / 2));
-        e = __ldg(p.x_scales + row * p.s_pitch + k / 32);
+    // moves n steps on; false when there are no more
+    auto move = [&](At& at, int n) {
+      at.st += n;
+      while (at.i < my_tiles && at.st >= at.tl.steps) {
+        at.st -= at.tl.steps;
+        if (++at.i < my_tiles) at.tl = tile_at(at.i);
       }
-      if (++lst == lt.steps) {
-        lst = 0;
-        ++li;
-        skip_empty();
-      }
+      return at.i < my_tiles;
     };
-    skip_empty();
+    uint4 codes[4];
+    uint32_t scale[4];
+    auto load = [&](const At& at) {
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) load(codes[j], scale[j]);
-    int gs = 0, i = 0, st = 0;
-    Tile tl = {};
-    auto next_tile = [&] {
-      while (i < my_tiles) {
-        tl = tile_at(i);
-        if (tl.steps > 0) break;
-        ++i;
-      }
-    };
-    next_tile();
-    bool ok = true;
-    while (ok && i < my_tiles) {
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        if (i >= my_tiles) break;
-        const int s = gs % kWgStages;
-        if (gs >= kWgStages && !mbar_wait_suspend(&empty[s], (uint32_t)((gs / kWgStages - 1) & 1))) {
-          atomicExch(failed, 1);
-          ok = false;
-          break;
+      for (int j = 0; j < 4; ++j) {
+        codes[j] = make_uint4(0u, 0u, 0u, 0u);
+        scale[j] = 127u;
+        const int in = at.st * kWgRows + r0 + 8 * j, k = at.tl.x0 + 32 * b;
+        if (in < at.tl.rows && k < p.K) {
+          const int64_t row = (int64_t)at.tl.row0 + in;
+          codes[j] = __ldg(reinterpret_cast<const uint4*>(p.x_codes + row * p.x_pitch + k / 2));
+          scale[j] = __ldg(p.x_scales + row * p.s_pitch + k / 32);
         }
+      }
+    };
+    At at{0, 0, {}};
+    if (my_tiles > 0) at.tl = tile_at(0);
+    bool more = move(at, first);
+    if (more) load(at);
+    for (int gs = first; more; gs += 4) {
+      const int s = gs % kWgStages;
+      uint8_t* stage = smem + s * kWgStage;
+      const int here = at.tl.rows - at.st * kWgRows;  // rows of the expert in this step
+      bool ok = gs < kWgStages || mbar_wait_suspend(&empty[s], (uint32_t)((gs / kWgStages - 1) & 1));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
         uint32_t v[16];
         expand32(codes[j], scale[j], v);
-        uint8_t* box = smem + s * kWgStage + (b >> 1) * kWgBox + r * 128;
+        const int r = r0 + 8 * j;
+        uint8_t* box = stage + (b >> 1) * kWgBox + r * 128;
+        if (ok) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<uint4*>(box + ((((b & 1) * 4 + q) ^ (r & 7)) << 4)) =
-              make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-        load(codes[j], scale[j]);
-        if (!mbar_wait_suspend(&dy_full[s], (uint32_t)((gs / kWgStages) & 1))) {
-          atomicExch(failed, 1);
-          ok = false;
-          break;
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<uint4*>(box + ((((b & 1) * 4 + q) ^ (r & 7)) << 4)) =
+                make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
         }
-        const int here = tl.rows - st * kWgRows;  // rows of the expert in this step
-        if (r >= here) {  // past its last: a row's four lanes clear its four half rows of dy
-          uint8_t* dyr = smem + s * kWgStage + kWgX + (b >> 1) * kWgBox + r * 128 + (b & 1) * 64;
+      }
+      more = move(at, 4);
+      if (more) load(at);
+      ok = ok && mbar_wait_suspend(&dy_full[s], (uint32_t)((gs / kWgStages) & 1));
+      if (!ok) {
+        atomicExch(failed, 1);
+        break;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = r0 + 8 * j;
+        if (r >= here) {  // past the expert's last row: its four lanes clear dy's four half rows
+          uint8_t* dyr = stage + kWgX + (b >> 1) * kWgBox + r * 128 + (b & 1) * 64;
 #pragma unroll
           for (int q = 0; q < 4; ++q)
             *reinterpret_cast<uint4*>(dyr + 16 * q) = make_uint4(0u, 0u, 0u, 0u);
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) peer_signal(full0 + 8 * s);
-        ++gs;
-        if (++st == tl.steps) {
-          st = 0;
-          ++i;
-          next_tile();
-        }
       }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) peer_signal(full0 + 8 * s);
     }
   }
   tc_fence_before();
