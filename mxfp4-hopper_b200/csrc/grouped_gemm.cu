@@ -690,7 +690,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) grouped_narrow_kernel(
         const Tile tl = tile_at(i);
         for (int ks = k_begin; ks < k_end; ++ks) {
           const int gs = issued, s = gs % kStages;
-          if (gs >= kStages && !mbar_wait(&empty[s], (uint32_t)((gs / kStages - 1) & 1))) {
+          if (gs >= kStages && !mbar_wait_suspend(&empty[s], (uint32_t)((gs / kStages - 1) & 1))) {
             atomicExch(failed, 1);
             ok = false;
             break;
@@ -715,27 +715,29 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) grouped_narrow_kernel(
       }
       // do not leave while copies of this CTA are still landing
       for (int gs = issued > kStages ? issued - kStages : 0; gs < issued; ++gs)
-        mbar_wait(&full[gs % kStages], (uint32_t)((gs / kStages) & 1));
+        mbar_wait_suspend(&full[gs % kStages], (uint32_t)((gs / kStages) & 1));
     }
   } else if (warp == 1) {
     // ------------------------------------------------ MMA issuer
-    if (lane == 0) {
+    {
+      const bool one = elect_one();
       bool ok = true;
       int gs = 0;
       for (int i = 0; ok && i < my_tiles; ++i) {
         const int buf = i & 1;
-        if (i > 1 && !mbar_wait(&acc_empty[buf], (uint32_t)((i / 2 - 1) & 1))) {
+        if (i > 1 && !mbar_wait_suspend(&acc_empty[buf], (uint32_t)((i / 2 - 1) & 1))) {
           ok = false;
           break;
         }
         tc_fence_after();
         for (int ks = k_begin; ks < k_end; ++ks, ++gs) {
           const int s = gs % kStages;
-          if (!mbar_wait(&full[s], (uint32_t)((gs / kStages) & 1))) {
+          if (!mbar_wait_suspend(&full[s], (uint32_t)((gs / kStages) & 1))) {
             ok = false;
             break;
           }
           tc_fence_after();
+          __syncwarp();
           const uint8_t* st = smem + s * L::kStage;
           const uint8_t* sf = st + kBlocks * kBoxBytes + kT * 128;
           const uint32_t sfw = tmem + kScaleCol + (uint32_t)s * L::kScaleCols;
@@ -746,8 +748,8 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) grouped_narrow_kernel(
             if (128 * a >= left) break;
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b)
-              tc_copy_sf(sfw + 8 * b + 4 * a, smem_desc_sf(sf + b * kAtoms + a * 512));
-            tc_copy_sf(sfr + 4 * a, smem_desc_sf(sf + kBlocks * kAtoms + a * 512));
+              tc_copy_sf(sfw + 8 * b + 4 * a, smem_desc_sf(sf + b * kAtoms + a * 512), one);
+            tc_copy_sf(sfr + 4 * a, smem_desc_sf(sf + kBlocks * kAtoms + a * 512), one);
           }
           const uint64_t dr = smem_desc_sw128(st + kBlocks * kBoxBytes);
 #pragma unroll
@@ -760,11 +762,12 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) grouped_narrow_kernel(
                      smem_desc_sw128(st + b * kBoxBytes) + (uint64_t)(2 * j),
                      dr + (uint64_t)(2 * j), mxf4_idesc(128, kT, sf_id),
                      (sfw + 8 * b + 4 * (j >> 1)) | (sf_id << 30),
-                     (sfr + 4 * (j >> 1)) | (sf_id << 30), (ks > k_begin || j > 0) ? 1u : 0u);
+                     (sfr + 4 * (j >> 1)) | (sf_id << 30), (ks > k_begin || j > 0) ? 1u : 0u, one);
           }
-          tc_commit(&empty[s]);
+          tc_commit(&empty[s], one);
         }
-        tc_commit(&acc_full[buf]);
+        __syncwarp();
+        tc_commit(&acc_full[buf], one);
       }
       if (!ok) atomicExch(failed, 1);
     }
@@ -779,7 +782,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) grouped_narrow_kernel(
       const Tile tl = tile_at(i);
       const int rows = min(kT, g.off[tl.e + 1] - tl.m0);
       const int buf = i & 1;
-      bool ok = mbar_wait(&acc_full[buf], (uint32_t)((i / 2) & 1));
+      bool ok = mbar_wait_suspend(&acc_full[buf], (uint32_t)((i / 2) & 1));
       // every owner has summed tile i - 1
       if (i > 0) ok = mbar_wait_cluster(part_empty, (uint32_t)((i - 1) & 1)) && ok;
       tc_fence_after();
@@ -879,7 +882,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) grouped_narrow_kernel(
           for (int j = 0; j < 4; ++j) {
             if (ks0 + j >= k_end) break;
             const int s = gs % kStages;
-            if (gs >= kStages && !mbar_wait(&empty[s], (uint32_t)((gs / kStages - 1) & 1))) {
+            if (gs >= kStages && !mbar_wait_suspend(&empty[s], (uint32_t)((gs / kStages - 1) & 1))) {
               atomicExch(failed, 1);
               ok = false;
               break;

@@ -215,6 +215,34 @@ __device__ __forceinline__ bool elect_one() {
   return r != 0;
 }
 
+// The MMA, scale copy and commit for a warp that runs converged, with `one` true in
+// one lane: the operands then stay in uniform registers (from a single-lane branch
+// each MMA took about 110 cycles to issue, more than it ran).
+__device__ __forceinline__ void tc_commit(uint64_t* bar, bool one) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(
+          smem_addr(bar)),
+      "r"((uint32_t)one)
+      : "memory");
+}
+__device__ __forceinline__ void tc_copy_sf(uint32_t taddr, uint64_t sdesc, bool one) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %2, 0;\n"
+      " @q tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n}" ::"r"(taddr),
+      "l"(sdesc), "r"((uint32_t)one)
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t sfa, uint32_t sfb, uint32_t accumulate, bool one) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %7, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::mxf4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6],"
+      " p;\n}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb), "r"((uint32_t)one)
+      : "memory");
+}
+
 // ---- two CTAs on one tile (cta_group::2): issued by the cluster's CTA 0
 // A TMA load into this CTA's shared memory whose bytes complete on a barrier of
 // CTA 0 (`bar`: its shared::cluster address).
@@ -237,10 +265,6 @@ __device__ __forceinline__ void tmem_dealloc_pair(uint32_t base, uint32_t cols) 
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(cols)
                : "memory");
 }
-// The issuing warp runs converged, with `one` true in one lane: the operands then
-// stay in uniform registers (from a single-lane branch each MMA took about 110
-// cycles to issue, more than it ran).
-//
 // Arrives on the barrier at this offset in both CTAs when the MMAs issued so far
 // have completed.
 __device__ __forceinline__ void tc_commit_pair(uint64_t* bar, bool one) {
