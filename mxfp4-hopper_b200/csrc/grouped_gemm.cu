@@ -51,81 +51,41 @@ struct GroupedArgs {
   int a_scales_tma;  // A's scales have a tensor map
 };
 
-// The rows' E8M0 bytes on their way to the tensor core: a thread has one row of
-// the tile and hands out its 8 bytes (the two words of its place in the step's two
-// atoms; zero past the row's S = K / 32 bytes) step by step.  Where the rows are
-// whole aligned words (K % 128 == 0 and a pitch of a multiple of 4) the next four
-// steps' words are in flight in registers; else each step's bytes are read when
-// they are due.
-template <typename TileAt>
-struct RowScales {
-  const GroupedArgs& p;
-  const TileAt& tile_at;
-  int r, begin, end, tiles;  // row in the tile, K steps, tiles of this CTA
-  bool words;
-  const uint8_t* src = nullptr;
-  bool in = false;
-  int ti = 0, ks = 0;
-  uint32_t next[8], now[8];
-
-  __device__ __forceinline__ void seek() {
-    ks = begin;
-    in = false;
-    if (ti < tiles && r >= 0) {
-      const int64_t row = (int64_t)tile_at(ti).m0 + r;
-      in = row < p.M;
-      src = p.a_scales + row * p.a_spitch;
-    }
-  }
-  __device__ __forceinline__ void fetch() {
-    const int S = p.K / 32;
+// E8M0 bytes b0 .. b0 + 31 (four K steps) of a warp's 32 rows -> dst[32][32] in
+// shared memory; zero past a row's S bytes and past the `rows` there are.  Whole
+// aligned words where the rows have them (4 rows an instruction), else a byte a
+// lane and a row an instruction: neighbouring lanes read neighbouring bytes either way.
+__device__ __forceinline__ void gather_scales(uint8_t* dst, const uint8_t* src, int64_t pitch,
+                                              int rows, int b0, int S, bool words) {
+  const int lane = threadIdx.x & 31;
+  if (words) {
+    const int at = b0 + 4 * (lane & 7);
+    uint32_t v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int at = ks * 8 + 4 * j;
-      next[j] = 0u;
-      if (words && in && at < S && ks + (j >> 1) < end)
-        next[j] = __ldg(reinterpret_cast<const uint32_t*>(src + at));
-    }
-  }
-  __device__ __forceinline__ RowScales(const GroupedArgs& p_, const TileAt& tile_at_, int r_,
-                                       int begin_, int end_, int tiles_)
-      : p(p_), tile_at(tile_at_), r(r_), begin(begin_), end(end_), tiles(tiles_) {
-    words = ((reinterpret_cast<uintptr_t>(p.a_scales) | (uintptr_t)p.a_spitch |
-              (uintptr_t)(p.K / 32)) & 3) == 0;
-    seek();
-    fetch();
-  }
-  // Takes the next four steps; they are handed out by get(0) .. get(3).
-  __device__ __forceinline__ void advance() {
-    if (!words) {
-      bytes_src = src;
-      bytes_in = in;
-      bytes_ks = ks;
+    for (int i = 0; i < 8; ++i) {
+      const int r = 4 * i + (lane >> 3);
+      v[i] = r < rows && at < S ? __ldg(reinterpret_cast<const uint32_t*>(src + r * pitch + at)) : 0u;
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) now[j] = next[j];
-    ks += 4;
-    if (ks >= end) {
-      ++ti;
-      seek();
+    for (int i = 0; i < 8; ++i)
+      *reinterpret_cast<uint32_t*>(dst + (4 * i + (lane >> 3)) * 32 + 4 * (lane & 7)) = v[i];
+  } else {
+#pragma unroll 1
+    for (int r0 = 0; r0 < 32; r0 += 16) {
+      uint32_t v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        v[i] = r0 + i < rows && b0 + lane < S ? __ldg(src + (r0 + i) * pitch + b0 + lane) : 0u;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dst[(r0 + i) * 32 + lane] = (uint8_t)v[i];
     }
-    fetch();
   }
-  __device__ __forceinline__ uint2 get(int j) const {
-    uint2 w = make_uint2(now[2 * j], now[2 * j + 1]);
-    if (!words && bytes_in) {
-      const int S = p.K / 32, b0 = (bytes_ks + j) * 8;
-      for (int i = 0; i < 4; ++i) {
-        if (b0 + i < S) w.x |= (uint32_t)bytes_src[b0 + i] << (8 * i);
-        if (b0 + 4 + i < S) w.y |= (uint32_t)bytes_src[b0 + 4 + i] << (8 * i);
-      }
-    }
-    return w;
-  }
-  const uint8_t* bytes_src = nullptr;
-  bool bytes_in = false;
-  int bytes_ks = 0;
-};
+}
+// Whether every row's scale bytes are whole aligned words.
+__device__ __forceinline__ bool scale_words(const GroupedArgs& p) {
+  return ((reinterpret_cast<uintptr_t>(p.a_scales) | (uintptr_t)p.a_spitch |
+           (uintptr_t)(p.K / 32)) & 3) == 0;
+}
 
 __device__ __forceinline__ float load_bias(const GroupedArgs& p, int64_t i) {
   return p.bias_f32 ? static_cast<const float*>(p.bias)[i]
@@ -351,22 +311,21 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
   } else if (warp < 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideScaleRegs));
     // ------------------------------------------------ scales
-    const int q = warp - 4, r = q * 32 + lane;
+    const int q = warp - 4;
     const uint32_t full0 = peer_addr(smem_addr(full), 0);
     const uint32_t col0 = tmem + ((uint32_t)(q * 32) << 16) + kScaleCol;
-    RowScales<decltype(tile_at)> rows(p, tile_at, r, 0, ksteps, p.a_scales_tma ? 0 : my_tiles);
+    const bool words = scale_words(p);
     int gs = 0, gq = 0;
     bool ok = true;
     for (int i = 0; ok && i < my_tiles; ++i) {
+      const int64_t row0 = p.a_scales_tma ? 0 : (int64_t)tile_at(i).m0 + 32 * q;
       for (int ks0 = 0; ok && ks0 < ksteps; ks0 += 4, ++gq) {
         const int sq = gq % kSbStages;
         uint8_t* sb = scales + sq * kSbStage;
         bool up = mbar_wait_suspend(&sb_full[sq], (uint32_t)((gq / kSbStages) & 1));
         if (!p.a_scales_tma) {
-          rows.advance();
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<uint2*>(sb + r * 32 + j * 8) = rows.get(j);
+          gather_scales(sb + 1024 * q, p.a_scales + row0 * p.a_spitch, p.a_spitch,
+                        (int)max((int64_t)0, min((int64_t)32, p.M - row0)), ks0 * 8, S, words);
           up = !named_sync_or(3, 128, !up);
         }
 #pragma unroll
@@ -421,7 +380,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
     // ------------------------------------------------ epilogue
     const int half = (warp - 8) >> 2, quad = warp & 3;
     const int r = quad * 32 + lane, ht = t & 127;
-    const bool issuer = ht == 0;
+    const bool issuer = ht < 32;  // the warp that issues the stores (its lane 0 does)
     uint8_t* boxes = out_boxes + half * kOutSlots * kOutBox;
     float* bias_h = bias_s + half * 128;
     constexpr int kHalfN = kTileN / 2;  // result columns of this group
@@ -547,9 +506,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
           named_sync(1 + half, 128);
           if (whole) {
             if (issuer) {
-              if (p.pre) tma_store_2d(&map_pre, n, tl.m0, bx);
-              if (kGlu && p.pre) tma_store_2d(&map_pre_up, n, tl.m0, bx + kOutBox);
-              if (p.c) tma_store_2d(&map_c, n, tl.m0, bx + n_pre * kOutBox);
+              __syncwarp();
+              if (p.pre) tma_store_2d(&map_pre, n, tl.m0, bx, lane == 0);
+              if (kGlu && p.pre) tma_store_2d(&map_pre_up, n, tl.m0, bx + kOutBox, lane == 0);
+              if (p.c) tma_store_2d(&map_c, n, tl.m0, bx + n_pre * kOutBox, lane == 0);
             }
           } else {
             // the group's last rows: only they are written
@@ -600,9 +560,11 @@ struct Narrow {
   static constexpr uint32_t kStage =
       kBlocks * (kBoxBytes + kAtoms) + (uint32_t)kT * 128 + kAtoms;
   static constexpr uint32_t kPart = kBlocks * kT * 128 * 4;  // partial sums, all ranks
-  static constexpr size_t kFixed = 1024 + kPart + kGroupTableInts * 4 + 512;
+  static constexpr size_t kFixed = 1024 + kPart + 2 * 1024 + kGroupTableInts * 4 + 512;
   static constexpr int kMost = (int)((227 * 1024 - kFixed) / kStage);
-  static constexpr int kStages = kMost > 9 ? 9 : kMost;
+  // Four stages: 128 rows over 32 experts of 4096 x 7168 take 77 us with 3 or 4, 81
+  // with the 5 that fit, and one row of 7168 x 2048 8.5 us with 4, 8.8 with 9.
+  static constexpr int kStages = kMost > 4 ? 4 : kMost;
   static constexpr size_t kSmem = kFixed + kStages * kStage;
   static constexpr uint32_t kScaleCols = kBlocks * 8 + 8;
   static_assert(kStages >= 3 && 2 * kBlocks * kT <= 256 && 256 + kStages * kScaleCols <= kTmemCols,
@@ -619,7 +581,8 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) grouped_narrow_kernel(
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
   float* part = reinterpret_cast<float*>(smem + kStages * L::kStage);
-  uint64_t* full = reinterpret_cast<uint64_t*>(part + L::kPart / 4);
+  uint8_t* row_bytes = reinterpret_cast<uint8_t*>(part + L::kPart / 4);  // 1 KB a scale warp
+  uint64_t* full = reinterpret_cast<uint64_t*>(row_bytes + 2 * 1024);
   uint64_t* empty = full + kStages;
   uint64_t* acc_full = empty + kStages;  // [2]
   uint64_t* acc_empty = acc_full + 2;    // [2]
@@ -872,12 +835,29 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) grouped_narrow_kernel(
     // ------------------------------------------------ the rows' scale bytes
     const int r = (warp - 6) * 32 + lane;
     if ((warp - 6) * 32 < kT) {
-      RowScales<decltype(tile_at)> mine(p, tile_at, r < kT ? r : -1, k_begin, k_end, my_tiles);
+      // The bytes of four steps are gathered through a scratch of this warp into
+      // registers, a row a thread.
+      const bool words = scale_words(p);
+      uint8_t* scratch = row_bytes + (warp - 6) * 1024;
+      uint4 next[2];
+      auto fetch = [&](const Tile& tl, int ks) {
+        const int64_t row0 = (int64_t)tl.m0 + (warp - 6) * 32;
+        __syncwarp();
+        gather_scales(scratch, p.a_scales + row0 * p.a_spitch, p.a_spitch,
+                      (int)max((int64_t)0, min((int64_t)min(32, kT - (warp - 6) * 32), p.M - row0)),
+                      ks * 8, S, words);
+        __syncwarp();
+        next[0] = *reinterpret_cast<const uint4*>(scratch + lane * 32);
+        next[1] = *reinterpret_cast<const uint4*>(scratch + lane * 32 + 16);
+      };
       int gs = 0;
       bool ok = true;
       for (int i = 0; ok && i < my_tiles; ++i) {
+        const Tile tl = tile_at(i);
         for (int ks0 = k_begin; ok && ks0 < k_end; ks0 += 4) {
-          mine.advance();
+          fetch(tl, ks0);
+          const uint32_t now[8] = {next[0].x, next[0].y, next[0].z, next[0].w,
+                                   next[1].x, next[1].y, next[1].z, next[1].w};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if (ks0 + j >= k_end) break;
@@ -889,9 +869,8 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) grouped_narrow_kernel(
             }
             uint8_t* sf = smem + s * L::kStage + kBlocks * (kBoxBytes + kAtoms) + kT * 128 +
                           lane * 16 + (warp - 6) * 4;
-            const uint2 w = mine.get(j);
-            *reinterpret_cast<uint32_t*>(sf) = w.x;
-            *reinterpret_cast<uint32_t*>(sf + 512) = w.y;
+            *reinterpret_cast<uint32_t*>(sf) = now[2 * j];
+            *reinterpret_cast<uint32_t*>(sf + 512) = now[2 * j + 1];
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&full[s]);
@@ -955,6 +934,8 @@ Plan grouped_plan(const GroupedArgs& p, bool glu) {
   r.tiles = most_tiles(p.M, p.E, r.rows, cdiv(p.width, 128));
   const int most = p.c_codes ? 4 : 8;  // a quantized block of 32 columns has one owner
   while (r.ranks < most && r.tiles * r.ranks * 2 <= sms && ksteps >= r.ranks * 4) r.ranks *= 2;
+  // long tiles in a few rounds: half tiles fill the last round better
+  if (r.ranks == 1 && ksteps >= 16 && r.tiles <= 8 * sms) r.ranks = 2;
   return r;
 }
 
