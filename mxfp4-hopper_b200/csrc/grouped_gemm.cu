@@ -87,6 +87,41 @@ __device__ __forceinline__ bool scale_words(const GroupedArgs& p) {
            (uintptr_t)(p.K / 32)) & 3) == 0;
 }
 
+// 32 BF16 columns of a row: in 32-byte sectors where base and pitch allow it, else in
+// 16-byte pieces; columns past the `cols` there are (a multiple of 8) are left alone.
+__device__ __forceinline__ bool sectors(const void* base, int64_t ld) {
+  return ((reinterpret_cast<uintptr_t>(base) | (uintptr_t)(ld * 2)) & 31) == 0;
+}
+__device__ __forceinline__ void store_cols(uint8_t* out, int cols, bool whole, const uint32_t (&w)[16]) {
+  if (whole && cols >= 32) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) st_v8(out + 32 * k, w + 8 * k);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (8 * k < cols)
+        *reinterpret_cast<uint4*>(out + 16 * k) =
+            make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+  }
+}
+__device__ __forceinline__ void load_cols(const uint8_t* src, int cols, bool whole, uint32_t (&w)[16]) {
+  if (whole && cols >= 32) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) ld_v8(src + 32 * k, w + 8 * k);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint4 x = make_uint4(0u, 0u, 0u, 0u);
+      if (8 * k < cols) x = __ldg(reinterpret_cast<const uint4*>(src + 16 * k));
+      w[4 * k] = x.x; w[4 * k + 1] = x.y; w[4 * k + 2] = x.z; w[4 * k + 3] = x.w;
+    }
+  }
+}
+__device__ __forceinline__ void pack32(const float* v, uint32_t (&w)[16]) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j) w[j] = cvt_bf16x2(v[2 * j], v[2 * j + 1]);
+}
+
 __device__ __forceinline__ float load_bias(const GroupedArgs& p, int64_t i) {
   return p.bias_f32 ? static_cast<const float*>(p.bias)[i]
                     : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[i]);
@@ -111,9 +146,10 @@ __device__ __forceinline__ float load_bias(const GroupedArgs& p, int64_t i) {
 //                a multiple of 16) are read by these warps, a row a thread
 //   warps 8-15   epilogue: two groups of four warps, each with half the columns.
 //                The accumulator is read into registers at once and given back,
-//                so that the next tile's products run under the epilogue
+//                so that the next tile's products run under the epilogue.  A
+//                thread has a row and writes it in whole 32-byte sectors
 constexpr int kWideThreads = 512;
-constexpr int kWideStages = 4;
+constexpr int kWideStages = 6;
 constexpr uint32_t kBoxBytes = 128 * 128;  // 128 rows of 128 code bytes
 constexpr uint32_t kAtoms = 2 * 512;       // scale atoms of 128 rows and one K step
 constexpr uint32_t kWideStage = 2 * kBoxBytes;
@@ -121,12 +157,10 @@ constexpr int kSbStages = 2;               // shared-memory scales of four steps
 constexpr uint32_t kSbA = 128 * 32;        // A's 128 rows of 32 bytes,
 constexpr uint32_t kSbB = 4 * kAtoms;      // 8 atoms of each of B's halves
 constexpr uint32_t kSbStage = kSbA + 2 * kSbB;
-constexpr uint32_t kOutBox = 128 * 64;     // 128 rows x 32 bf16 columns, 64-byte swizzle
-constexpr int kOutSlots = 4;               // per epilogue group
 constexpr uint32_t kScaleCol = 256;        // tensor memory: accumulator, then scales
 constexpr uint32_t kTmemCols = 512;
-constexpr size_t kWideSmem = 1024 + kWideStages * kWideStage + kSbStages * kSbStage +
-                             2 * kOutSlots * kOutBox + 256 * 4 + kGroupTableInts * 4 + 512;
+constexpr size_t kWideSmem = 1024 + kWideStages * kWideStage + kSbStages * kSbStage + 256 * 4 +
+                             kGroupTableInts * 4 + 512;
 static_assert(kWideSmem <= 227 * 1024, "one CTA per SM");
 static_assert(kScaleCol + 24 * kWideStages <= kTmemCols, "scales fit beside the accumulator");
 static_assert(kWideStage % 1024 == 0, "swizzled boxes start on 1024 bytes");
@@ -137,16 +171,13 @@ constexpr int kWideCopyRegs = 64, kWideScaleRegs = 96, kWideEpilogueRegs = 176;
 template <int kAct>
 __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
     const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-    const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_c,
-    const __grid_constant__ CUtensorMap map_pre, const __grid_constant__ CUtensorMap map_pre_up,
-    const __grid_constant__ GroupedArgs p) {
+    const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ GroupedArgs p) {
   constexpr bool kGlu = kAct == MXB_ACT_SWIGLU;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
   uint8_t* scales = smem + kWideStages * kWideStage;
-  uint8_t* out_boxes = scales + kSbStages * kSbStage;
-  float* bias_s = reinterpret_cast<float*>(out_boxes + 2 * kOutSlots * kOutBox);
+  float* bias_s = reinterpret_cast<float*>(scales + kSbStages * kSbStage);
   // CTA 0's: a step's codes of both CTAs have landed and its scales are in tensor memory
   uint64_t* full = reinterpret_cast<uint64_t*>(bias_s + 256);
   uint64_t* empty = full + kWideStages;
@@ -380,20 +411,17 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
     // ------------------------------------------------ epilogue
     const int half = (warp - 8) >> 2, quad = warp & 3;
     const int r = quad * 32 + lane, ht = t & 127;
-    const bool issuer = ht < 32;  // the warp that issues the stores (its lane 0 does)
-    uint8_t* boxes = out_boxes + half * kOutSlots * kOutBox;
     float* bias_h = bias_s + half * 128;
     constexpr int kHalfN = kTileN / 2;  // result columns of this group
-    const int n_pre = p.pre ? (kGlu ? 2 : 1) : 0;
-    const int n_box = n_pre + (p.c ? 1 : 0);
-    const int sets = n_box == 3 ? 1 : n_box == 2 ? 2 : 4;
     const uint32_t acc_empty0 = peer_addr(smem_addr(acc_empty), 0);
     const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
-    int set = 0;
+    const bool c32 = sectors(p.c, p.c_ld), pre32 = sectors(p.pre, p.pre_ld) && p.width % 16 == 0;
+    const bool res32 = sectors(p.residual, p.residual_ld);
     for (int i = 0; i < my_tiles; ++i) {
       const Tile tl = tile_at(i);
       const int rows = min(128, g.off[tl.e + 1] - tl.m0);  // none or fewer: CTA 1's share
       const int nh = tl.n0 + half * kHalfN;                // first result column of this group
+      const bool mine = r < rows;
       float bias = 0.0f;
       if (p.bias) {
         // this group's 128 accumulator columns: 128 of z, or 64 gate and 64 up
@@ -402,19 +430,14 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
                                 : (int64_t)tl.e * p.width + col;
         if (col < p.width) bias = load_bias(p, at);
       }
+      named_sync(1 + half, 128);  // the tile before has read its bias
       bias_h[ht] = bias;
-      const bool whole = rows == 128;
       const int64_t row = (int64_t)tl.m0 + r;
       // this row's residual of one chunk of 32 columns, read a chunk ahead
-      uint4 res[4];
+      uint32_t res[16];
       auto load_residual = [&](int n) {
-        const uint8_t* src = p.residual + (row * p.residual_ld + n) * 2;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          res[k] = make_uint4(0u, 0u, 0u, 0u);
-          if (p.residual && r < rows && n + 8 * k < p.width)
-            res[k] = __ldg(reinterpret_cast<const uint4*>(src + 16 * k));
-        }
+        if (p.residual && mine && n < p.width)
+          load_cols(p.residual + (row * p.residual_ld + n) * 2, p.width - n, res32, res);
       };
       load_residual(nh);
       const bool ok = mbar_wait_suspend(acc_full, (uint32_t)(i & 1));
@@ -432,107 +455,70 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
       tc_fence_before();
       __syncwarp();
       if (lane == 0) peer_signal(acc_empty0);
-      if (rows <= 0) continue;
-      // One copy of the code for all chunks (unrolled four times it runs from beyond
-      // the instruction caches, at half the rate): the registers move down instead.
+      if (!mine) continue;
+      // One copy of the code for all chunks of 32 columns: the registers move down.
 #pragma unroll 1
       for (int ch = 0; ch < kHalfN / 32; ++ch) {
-        const int n = nh + 32 * ch;
-        if (n >= p.width) break;
-        {
-          float v[32], u[kGlu ? 32 : 1];
-          auto add_bias = [&](const uint32_t* a, const float* b, float* z) {
+        const int n = nh + 32 * ch, cols = p.width - n;
+        if (cols <= 0) break;
+        float v[32], u[kGlu ? 32 : 1];
+        auto add_bias = [&](const uint32_t* a, const float* b, float* z) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              const float4 w = *reinterpret_cast<const float4*>(b + j);
-              add2(F2(__uint_as_float(a[j]), __uint_as_float(a[j + 1])), F2(w.x, w.y)).get(z[j], z[j + 1]);
-              add2(F2(__uint_as_float(a[j + 2]), __uint_as_float(a[j + 3])), F2(w.z, w.w)).get(z[j + 2], z[j + 3]);
-            }
-          };
-          add_bias(acc, bias_h + 32 * ch, v);
-          if constexpr (kGlu) add_bias(acc + 64, bias_h + 64 + 32 * ch, u);
+          for (int j = 0; j < 32; j += 4) {
+            const float4 w = *reinterpret_cast<const float4*>(b + j);
+            add2(F2(__uint_as_float(a[j]), __uint_as_float(a[j + 1])), F2(w.x, w.y)).get(z[j], z[j + 1]);
+            add2(F2(__uint_as_float(a[j + 2]), __uint_as_float(a[j + 3])), F2(w.z, w.w)).get(z[j + 2], z[j + 3]);
+          }
+        };
+        add_bias(acc, bias_h + 32 * ch, v);
+        if constexpr (kGlu) {
+          add_bias(acc + 64, bias_h + 64 + 32 * ch, u);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            acc[j] = acc[32 + j];
+            acc[64 + j] = acc[96 + j];
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 96; ++j) acc[j] = acc[32 + j];
+        }
+        uint32_t w[16];
+        if (p.pre) {
+          uint8_t* out = p.pre + (row * p.pre_ld + n) * 2;
+          pack32(v, w);
+          store_cols(out, cols, pre32, w);
           if constexpr (kGlu) {
+            pack32(u, w);
+            store_cols(out + (int64_t)p.width * 2, cols, pre32, w);
+          }
+        }
+        if constexpr (kGlu) {
+          act_each<MXB_ACT_SILU>(v);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              acc[j] = acc[32 + j];
-              acc[64 + j] = acc[96 + j];
-            }
-          } else {
+          for (int j = 0; j < 32; j += 2)
+            mul2(F2(v[j], v[j + 1]), F2(u[j], u[j + 1])).get(v[j], v[j + 1]);
+        } else {
+          act_each<kAct>(v);
+        }
+        if (p.residual) {
 #pragma unroll
-            for (int j = 0; j < 96; ++j) acc[j] = acc[32 + j];
+          for (int j = 0; j < 16; ++j) {
+            v[2 * j] += bf16lo_to_f(res[j]);
+            v[2 * j + 1] += bf16hi_to_f(res[j]);
           }
-          // the boxes of this set have been read by the stores issued `sets` chunks ago
-          if (issuer) {
-            if (sets == 1) bulk_wait_read_all();
-            else if (sets == 2) bulk_wait_read_1();
-            else bulk_wait_read_3();
-          }
-          named_sync(1 + half, 128);
-          uint8_t* bx = boxes + set * n_box * kOutBox;
-          auto put = [&](uint8_t* box, const float* x) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              *reinterpret_cast<uint4*>(box + r * 64 + ((k ^ ((r >> 1) & 3)) << 4)) =
-                  pack8_bf16(x + 8 * k);
-          };
-          if (p.pre) {
-            put(bx, v);
-            if constexpr (kGlu) put(bx + kOutBox, u);
-          }
-          if constexpr (kGlu) {
-            act_each<MXB_ACT_SILU>(v);
-#pragma unroll
-            for (int j = 0; j < 32; j += 2)
-              mul2(F2(v[j], v[j + 1]), F2(u[j], u[j + 1])).get(v[j], v[j + 1]);
-          } else {
-            act_each<kAct>(v);
-          }
-          if (p.residual) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) add8_bf16(v + 8 * k, res[k]);
-            if (32 * (ch + 1) < kHalfN) load_residual(n + 32);
-          }
-          if (p.c) put(bx + n_pre * kOutBox, v);
-          if (p.c_codes && r < rows) {
-            uint32_t w[16], q[4], byte;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) w[j] = cvt_bf16x2(v[2 * j], v[2 * j + 1]);
-            quant_block32<true>(w, QuantParams{1e-10f, -6.0f, 6.0f}, q, byte);
-            *reinterpret_cast<uint4*>(p.c_codes + (row * p.width + n) / 2) =
-                make_uint4(q[0], q[1], q[2], q[3]);
-            p.c_scales[(row * p.width + n) / 32] = (uint8_t)byte;
-          }
-          if (whole) fence_proxy_async_smem();
-          named_sync(1 + half, 128);
-          if (whole) {
-            if (issuer) {
-              __syncwarp();
-              if (p.pre) tma_store_2d(&map_pre, n, tl.m0, bx, lane == 0);
-              if (kGlu && p.pre) tma_store_2d(&map_pre_up, n, tl.m0, bx + kOutBox, lane == 0);
-              if (p.c) tma_store_2d(&map_c, n, tl.m0, bx + n_pre * kOutBox, lane == 0);
-            }
-          } else {
-            // the group's last rows: only they are written
-            auto copy = [&](const uint8_t* box, uint8_t* out, int64_t ld) {
-              for (int x = ht; x < rows * 4; x += 128) {
-                const int rr = x >> 2, k = x & 3;
-                if (n + 8 * k < p.width)
-                  *reinterpret_cast<uint4*>(out + (((int64_t)tl.m0 + rr) * ld + n + 8 * k) * 2) =
-                      *reinterpret_cast<const uint4*>(box + rr * 64 + ((k ^ ((rr >> 1) & 3)) << 4));
-              }
-            };
-            if (p.pre) {
-              copy(bx, p.pre, p.pre_ld);
-              if (kGlu) copy(bx + kOutBox, p.pre + (int64_t)p.width * 2, p.pre_ld);
-            }
-            if (p.c) copy(bx + n_pre * kOutBox, p.c, p.c_ld);
-          }
-          if (issuer) bulk_commit();  // an empty group where nothing was stored
-          set = set + 1 == sets ? 0 : set + 1;
+          if (ch + 1 < kHalfN / 32) load_residual(n + 32);
+        }
+        pack32(v, w);
+        if (p.c) store_cols(p.c + (row * p.c_ld + n) * 2, cols, c32, w);
+        if (p.c_codes) {
+          uint32_t q[4], byte;
+          quant_block32<true>(w, QuantParams{1e-10f, -6.0f, 6.0f}, q, byte);
+          *reinterpret_cast<uint4*>(p.c_codes + (row * p.width + n) / 2) =
+              make_uint4(q[0], q[1], q[2], q[3]);
+          p.c_scales[(row * p.width + n) / 32] = (uint8_t)byte;
         }
       }
     }
-    if (issuer) bulk_wait_all();
   }
   tc_fence_before();
   __syncthreads();
@@ -833,7 +819,6 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) grouped_narrow_kernel(
     }
   } else {
     // ------------------------------------------------ the rows' scale bytes
-    const int r = (warp - 6) * 32 + lane;
     if ((warp - 6) * 32 < kT) {
       // The bytes of four steps are gathered through a scratch of this warp into
       // registers, a row a thread.
@@ -930,25 +915,25 @@ Plan grouped_plan(const GroupedArgs& p, bool glu) {
   const int64_t wide = most_tiles(p.M, p.E, 256, cdiv(p.width, glu ? 128 : 256));
   Plan r{256, 1, wide};
   if (p.M > 96 * (int64_t)p.E && wide >= sms / 2) return r;
-  r.rows = p.M <= 24 * (int64_t)p.E ? 16 : 64;
+  r.rows = p.M <= 8 * (int64_t)p.E ? 16 : 64;
   r.tiles = most_tiles(p.M, p.E, r.rows, cdiv(p.width, 128));
   const int most = p.c_codes ? 4 : 8;  // a quantized block of 32 columns has one owner
   while (r.ranks < most && r.tiles * r.ranks * 2 <= sms && ksteps >= r.ranks * 4) r.ranks *= 2;
-  // long tiles in a few rounds: half tiles fill the last round better
-  if (r.ranks == 1 && ksteps >= 16 && r.tiles <= 8 * sms) r.ranks = 2;
+  // long tiles in a few rounds that read each weight for a few rows: half tiles fill
+  // the last round better
+  if (r.ranks == 1 && ksteps >= 16 && p.M <= 32 * (int64_t)p.E && r.tiles <= 8 * sms) r.ranks = 2;
   return r;
 }
 
 template <int kAct>
 mxb_status launch_wide(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& ts,
-                       const CUtensorMap& tc, const CUtensorMap& tp, const CUtensorMap& tu,
                        const GroupedArgs& p, const Plan& plan, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
   MXB_REQUIRE(grant_smem((const void*)grouped_wide_kernel<kAct>, kWideSmem, done), MXB_ERR_CUDA,
               "grouped_gemm_mxfp4: cannot reserve shared memory");
   return launch_cluster("grouped_gemm_mxfp4", grouped_wide_kernel<kAct>,
                         (unsigned)std::min<int64_t>(plan.tiles, std::max(1, sm_count() / 2)), 2,
-                        kWideThreads, kWideSmem, s, ta, tb, ts, tc, tp, tu, p);
+                        kWideThreads, kWideSmem, s, ta, tb, ts, p);
 }
 
 template <bool kGlu, int kT>
@@ -1071,22 +1056,13 @@ extern "C" mxb_status mxb_grouped_gemm_mxfp4(const void* a_codes, int64_t a_code
   if (p.a_scales_tma && !make_tensor_map_2d(&ts, a_scales, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, M,
                                             K / 32, a_scales_pitch, 32, 128))
     return MXB_ERR_CUDA;
-  // output maps are one part wide, so that a box never reaches into the other part
-  CUtensorMap tc = ta, tp = ta, tu = ta;
-  auto out_map = [&](CUtensorMap* m, void* base, int64_t ld) {
-    return make_tensor_map_2d(m, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, M, W, ld, 32, 128,
-                              CU_TENSOR_MAP_SWIZZLE_64B);
-  };
-  if ((c && !out_map(&tc, c, ep->c_ld)) || (ep->pre && !out_map(&tp, ep->pre, ep->pre_ld)) ||
-      (ep->pre && glu && !out_map(&tu, (uint8_t*)ep->pre + W * 2, ep->pre_ld)))
-    return MXB_ERR_CUDA;
   switch (p.act) {
-    case MXB_ACT_RELU: return launch_wide<MXB_ACT_RELU>(ta, tb, ts, tc, tp, tu, p, plan, s);
-    case MXB_ACT_RELU2: return launch_wide<MXB_ACT_RELU2>(ta, tb, ts, tc, tp, tu, p, plan, s);
-    case MXB_ACT_SILU: return launch_wide<MXB_ACT_SILU>(ta, tb, ts, tc, tp, tu, p, plan, s);
-    case MXB_ACT_GELU: return launch_wide<MXB_ACT_GELU>(ta, tb, ts, tc, tp, tu, p, plan, s);
-    case MXB_ACT_GELU_TANH: return launch_wide<MXB_ACT_GELU_TANH>(ta, tb, ts, tc, tp, tu, p, plan, s);
-    case MXB_ACT_SWIGLU: return launch_wide<MXB_ACT_SWIGLU>(ta, tb, ts, tc, tp, tu, p, plan, s);
-    default: return launch_wide<MXB_ACT_NONE>(ta, tb, ts, tc, tp, tu, p, plan, s);
+    case MXB_ACT_RELU: return launch_wide<MXB_ACT_RELU>(ta, tb, ts, p, plan, s);
+    case MXB_ACT_RELU2: return launch_wide<MXB_ACT_RELU2>(ta, tb, ts, p, plan, s);
+    case MXB_ACT_SILU: return launch_wide<MXB_ACT_SILU>(ta, tb, ts, p, plan, s);
+    case MXB_ACT_GELU: return launch_wide<MXB_ACT_GELU>(ta, tb, ts, p, plan, s);
+    case MXB_ACT_GELU_TANH: return launch_wide<MXB_ACT_GELU_TANH>(ta, tb, ts, p, plan, s);
+    case MXB_ACT_SWIGLU: return launch_wide<MXB_ACT_SWIGLU>(ta, tb, ts, p, plan, s);
+    default: return launch_wide<MXB_ACT_NONE>(ta, tb, ts, p, plan, s);
   }
 }

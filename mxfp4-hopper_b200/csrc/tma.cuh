@@ -157,18 +157,6 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int32_t x, 
       "r"(x), "r"(y), "r"(smem_addr(src))
       : "memory");
 }
-// The same from a warp that runs converged, issued by the lane with `one` true (the
-// operands stay in uniform registers: from a single-lane branch a store took about
-// 700 cycles to issue).
-__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int32_t x, int32_t y,
-                                             const void* src, bool one) {
-  asm volatile(
-      "{\n .reg .pred q;\n setp.ne.b32 q, %4, 0;\n"
-      " @q cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];\n}" ::"l"(
-          reinterpret_cast<uint64_t>(map)),
-      "r"(x), "r"(y), "r"(smem_addr(src)), "r"((uint32_t)one)
-      : "memory");
-}
 // 1-D bulk copy of `bytes` contiguous bytes shared -> global (bulk group).
 // Both addresses 16-byte aligned, bytes a multiple of 16.
 __device__ __forceinline__ void bulk_store_1d(void* dst, const void* src, uint32_t bytes) {
@@ -187,10 +175,6 @@ __device__ __forceinline__ void bulk_wait_read_all() {
 // Waits until at most one committed bulk store group is still reading shared memory.
 __device__ __forceinline__ void bulk_wait_read_1() {
   asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-}
-// Waits until at most three committed bulk store groups are still reading shared memory.
-__device__ __forceinline__ void bulk_wait_read_3() {
-  asm volatile("cp.async.bulk.wait_group.read 3;" ::: "memory");
 }
 // Waits until every committed bulk store has completed.
 __device__ __forceinline__ void bulk_wait_all() {
