@@ -83,27 +83,6 @@ __device__ __forceinline__ float act_value(float z) {
   return z;
 }
 
-// d act / d z
-template <int kAct>
-__device__ __forceinline__ float act_slope(float z) {
-  if constexpr (kAct == MXB_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
-  if constexpr (kAct == MXB_ACT_RELU2) return z > 0.0f ? 2.0f * z : 0.0f;
-  if constexpr (kAct == MXB_ACT_SILU) {
-    const float s = logistic(z);
-    return s * (1.0f + z * (1.0f - s));
-  }
-  if constexpr (kAct == MXB_ACT_GELU) {
-    float gauss;
-    const float q = normal_tail(z, gauss);
-    return (z > 0.0f ? 1.0f - q : q) + z * kInvSqrt2Pi * gauss;
-  }
-  if constexpr (kAct == MXB_ACT_GELU_TANH) {
-    const float s = logistic(2.0f * kSqrt2OverPi * (z + kGeluCubic * z * z * z));
-    return s + z * s * (1.0f - s) * 2.0f * kSqrt2OverPi * (1.0f + 3.0f * kGeluCubic * z * z);
-  }
-  return 1.0f;
-}
-
 // Two floats in a register pair, for the packed f32 instructions.
 struct F2 {
   uint64_t v;
@@ -149,6 +128,43 @@ __device__ __forceinline__ void logistic_pairs(const F2 (&z)[kP], F2 (&s)[kP]) {
   }
 }
 
+// normal_tail() of kP pairs, as the factor of gelu: 1 - q where z > 0, else q.
+template <int kP>
+__device__ __forceinline__ void normal_cdf_pairs(const float* v, const F2 (&z)[kP], F2 (&cdf)[kP],
+                                                 F2 (&gauss)[kP]) {
+  F2 t[kP];
+#pragma unroll
+  for (int i = 0; i < kP; ++i) {
+    float a, b;
+    fma2(F2(fabsf(v[2 * i]), fabsf(v[2 * i + 1])), both(0.3f), both(1.0f)).get(a, b);
+    t[i] = F2(rcp_approx(a), rcp_approx(b));
+  }
+#pragma unroll
+  for (int i = 0; i < kP; ++i) {
+    float a, b;
+    mul2(mul2(z[i], z[i]), both(-0.5f * kLog2e)).get(a, b);
+    gauss[i] = F2(ex2_approx(a), ex2_approx(b));
+  }
+#pragma unroll
+  for (int i = 0; i < kP; ++i) cdf[i] = fma2(both(tail_coeff(7)), t[i], both(tail_coeff(6)));
+#pragma unroll
+  for (int c = 5; c >= 0; --c)
+#pragma unroll
+    for (int i = 0; i < kP; ++i) cdf[i] = fma2(cdf[i], t[i], both(tail_coeff(c)));
+#pragma unroll
+  for (int i = 0; i < kP; ++i) {
+    const F2 q = mul2(mul2(cdf[i], t[i]), gauss[i]);
+    float q0, q1, r0, r1;
+    q.get(q0, q1);
+    fma2(q, both(-1.0f), both(1.0f)).get(r0, r1);
+    cdf[i] = F2(v[2 * i] > 0.0f ? r0 : q0, v[2 * i + 1] > 0.0f ? r1 : q1);
+  }
+}
+// 2 u of gelu_tanh: 2 sqrt(2 / pi) (z + 0.044715 z^3).
+__device__ __forceinline__ F2 tanh_arg(F2 z) {
+  return mul2(fma2(mul2(z, both(kGeluCubic)), mul2(z, z), z), both(2.0f * kSqrt2OverPi));
+}
+
 // Eight values at a time, step by step and in pairs: a value alone is a chain of
 // dependent instructions (about 110 cycles for gelu), and the epilogue has two
 // warps a scheduler to hide it with.  The same arithmetic as act_value(), in
@@ -156,55 +172,68 @@ __device__ __forceinline__ void logistic_pairs(const F2 (&z)[kP], F2 (&s)[kP]) {
 template <int kAct>
 __device__ __forceinline__ void act8(float* v) {
   constexpr int kP = 4;
-  F2 z[kP], s[kP];
   if constexpr (kAct == MXB_ACT_SILU || kAct == MXB_ACT_GELU || kAct == MXB_ACT_GELU_TANH) {
+    F2 z[kP], s[kP];
 #pragma unroll
     for (int i = 0; i < kP; ++i) z[i] = F2(v[2 * i], v[2 * i + 1]);
-  }
-  if constexpr (kAct == MXB_ACT_SILU) {
-    logistic_pairs<kP>(z, s);
-  } else if constexpr (kAct == MXB_ACT_GELU_TANH) {
-    F2 u[kP];
+    if constexpr (kAct == MXB_ACT_SILU) {
+      logistic_pairs<kP>(z, s);
+    } else if constexpr (kAct == MXB_ACT_GELU_TANH) {
+      F2 u[kP];
 #pragma unroll
-    for (int i = 0; i < kP; ++i)
-      u[i] = mul2(fma2(mul2(z[i], both(kGeluCubic)), mul2(z[i], z[i]), z[i]),
-                  both(2.0f * kSqrt2OverPi));
-    logistic_pairs<kP>(u, s);
-  } else if constexpr (kAct == MXB_ACT_GELU) {
-    F2 t[kP], g[kP];
-#pragma unroll
-    for (int i = 0; i < kP; ++i) {
-      float a, b;
-      fma2(F2(fabsf(v[2 * i]), fabsf(v[2 * i + 1])), both(0.3f), both(1.0f)).get(a, b);
-      t[i] = F2(rcp_approx(a), rcp_approx(b));
+      for (int i = 0; i < kP; ++i) u[i] = tanh_arg(z[i]);
+      logistic_pairs<kP>(u, s);
+    } else {
+      F2 gauss[kP];
+      normal_cdf_pairs<kP>(v, z, s, gauss);
     }
-#pragma unroll
-    for (int i = 0; i < kP; ++i) {
-      float a, b;
-      mul2(mul2(z[i], z[i]), both(-0.5f * kLog2e)).get(a, b);
-      g[i] = F2(ex2_approx(a), ex2_approx(b));
-    }
-#pragma unroll
-    for (int i = 0; i < kP; ++i) s[i] = fma2(both(tail_coeff(7)), t[i], both(tail_coeff(6)));
-#pragma unroll
-    for (int c = 5; c >= 0; --c)
-#pragma unroll
-      for (int i = 0; i < kP; ++i) s[i] = fma2(s[i], t[i], both(tail_coeff(c)));
-#pragma unroll
-    for (int i = 0; i < kP; ++i) {
-      const F2 q = mul2(mul2(s[i], t[i]), g[i]);
-      float q0, q1, r0, r1;
-      q.get(q0, q1);
-      fma2(q, both(-1.0f), both(1.0f)).get(r0, r1);
-      s[i] = F2(v[2 * i] > 0.0f ? r0 : q0, v[2 * i + 1] > 0.0f ? r1 : q1);
-    }
-  }
-  if constexpr (kAct == MXB_ACT_SILU || kAct == MXB_ACT_GELU || kAct == MXB_ACT_GELU_TANH) {
 #pragma unroll
     for (int i = 0; i < kP; ++i) mul2(z[i], s[i]).get(v[2 * i], v[2 * i + 1]);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = act_value<kAct>(v[i]);
+  }
+}
+// The derivatives of eight values, likewise: with s the logistic (or normal)
+// factor, silu s + z s (1 - s), gelu_tanh s + z s (1 - s) d(2u)/dz, gelu s + z times
+// the normal density.
+template <int kAct>
+__device__ __forceinline__ void slope8(const float* v, float* out) {
+  constexpr int kP = 4;
+  if constexpr (kAct == MXB_ACT_SILU || kAct == MXB_ACT_GELU || kAct == MXB_ACT_GELU_TANH) {
+    F2 z[kP], s[kP], o[kP];
+#pragma unroll
+    for (int i = 0; i < kP; ++i) z[i] = F2(v[2 * i], v[2 * i + 1]);
+    if constexpr (kAct == MXB_ACT_GELU) {
+      F2 gauss[kP];
+      normal_cdf_pairs<kP>(v, z, s, gauss);
+#pragma unroll
+      for (int i = 0; i < kP; ++i) o[i] = fma2(mul2(z[i], both(kInvSqrt2Pi)), gauss[i], s[i]);
+    } else {
+      if constexpr (kAct == MXB_ACT_SILU) {
+        logistic_pairs<kP>(z, s);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kP; ++i) o[i] = tanh_arg(z[i]);
+        logistic_pairs<kP>(o, s);
+      }
+#pragma unroll
+      for (int i = 0; i < kP; ++i) {
+        F2 zs = mul2(z[i], s[i]);
+        if constexpr (kAct == MXB_ACT_GELU_TANH)
+          zs = mul2(zs, fma2(mul2(z[i], z[i]), both(6.0f * kSqrt2OverPi * kGeluCubic),
+                             both(2.0f * kSqrt2OverPi)));
+        o[i] = fma2(zs, fma2(s[i], both(-1.0f), both(1.0f)), s[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kP; ++i) o[i].get(out[2 * i], out[2 * i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      out[i] = kAct == MXB_ACT_RELU    ? (v[i] > 0.0f ? 1.0f : 0.0f)
+               : kAct == MXB_ACT_RELU2 ? (v[i] > 0.0f ? 2.0f * v[i] : 0.0f)
+                                       : 1.0f;
   }
 }
 template <int kAct, int n>

@@ -18,48 +18,56 @@ namespace mxb {
 namespace {
 
 // ---------------------------------------------------------------- bias_act_grad
-// A CTA takes kGradRows rows of one expert by 256 columns of dy: a warp a row, a
-// lane eight columns, four rows in flight.  Column sums stay in registers over a
+// A CTA takes up to 128 rows of one expert by 256 columns of dy: a warp a row, a
+// lane eight columns.  Column sums stay in registers over a
 // warp's rows, meet in shared memory in warp order, and leave as one partial sum
 // per CTA; a second kernel adds an expert's partials in row order, so the bias
-// gradient does not depend on scheduling.  With at most kGradRows rows there is
-// one CTA per expert and column range, which writes dbias itself.
-constexpr int kGradRows = 128;
+// gradient does not depend on scheduling.  Where all rows fit one CTA's share there
+// is one CTA per expert and column range, which writes dbias itself.
 constexpr int kGradThreads = 256, kGradWarps = 8, kGradCols = 256;
 
-__device__ __forceinline__ int grad_chunks(int rows) {
-  return rows > kGradRows ? (rows + kGradRows - 1) / kGradRows : 1;
+// Rows of a CTA: fewer where 128 would leave SMs without work (333 x 1024: 10.5 us
+// with 128, 5.9 with 32).
+int grad_rows(int64_t M, int64_t N) {
+  return (M / 128) * cdiv(N, kGradCols) >= 2 * kSMs ? 128 : 32;
 }
-int64_t most_grad_chunks(int64_t M, int64_t E) { return M / kGradRows + E; }
+__device__ __forceinline__ int grad_chunks(int rows, int per) {
+  return rows > per ? (rows + per - 1) / per : 1;
+}
+int64_t most_grad_chunks(int64_t M, int64_t E, int per) { return M / per + E; }
 
 struct ActGradArgs {
   const uint8_t *dy, *pre;
   const int32_t* m_splits;
   int64_t M;
-  int E, N, width;
+  int E, N, width, per;  // per: rows of a CTA
   uint8_t *dz, *codes, *scales;
   float* sums;  // [chunks, N] partials, or dbias itself; NULL: no bias gradient
 };
 
-template <int kAct>
-__global__ void __launch_bounds__(kGradThreads) act_grad_kernel(const ActGradArgs p, int slabs) {
+// Bytes in flight come from many warps with few rows each: swiglu 16384 x 8192 took
+// 148 us with four rows a thread and one CTA per SM, 128 with two and two, 119 with
+// one row and three CTAs; gelu of the same size 253, 167 and (two rows, three CTAs) 141.
+template <int kAct, bool kQuant>
+__global__ void __launch_bounds__(kGradThreads, kQuant ? 2 : 3)
+    act_grad_kernel(const ActGradArgs p, int slabs) {
   constexpr bool kGlu = kAct == MXB_ACT_SWIGLU;
   constexpr int kParts = kGlu ? 2 : 1;
   __shared__ int32_t table[kGroupTableInts];
   __shared__ float red[kParts][kGradWarps][kGradCols];
   const GroupTable g{table, table + p.E + 1};
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-  if (warp == 0) build_groups(g, p.m_splits, p.E, p.M, grad_chunks);
+  if (warp == 0) build_groups(g, p.m_splits, p.E, p.M, [&](int rows) { return grad_chunks(rows, p.per); });
   __syncthreads();
   const int chunk = (int)(blockIdx.x / slabs), slab = (int)(blockIdx.x % slabs);
   if (chunk >= g.tile[p.E]) return;
   const int e = find_group(g.tile, p.E, chunk);
-  const int r0 = g.off[e] + (chunk - g.tile[e]) * kGradRows;
-  const int r1 = min(r0 + kGradRows, g.off[e + 1]);
+  const int r0 = g.off[e] + (chunk - g.tile[e]) * p.per;
+  const int r1 = min(r0 + p.per, g.off[e + 1]);
   const int n = slab * kGradCols + lane * 8;
   const bool in = n < p.width;
   float sum[kParts][8] = {};
-  constexpr int kRows = 4;
+  constexpr int kRows = kGlu ? 1 : 2;
   for (int r = r0 + warp; r < r1; r += kGradWarps * kRows) {
     uint4 d[kRows], z[kParts][kRows];
 #pragma unroll
@@ -85,17 +93,23 @@ __global__ void __launch_bounds__(kGradThreads) act_grad_kernel(const ActGradArg
           float a[8], b[8];
           unpack8_bf16(z[0][q], a);
           unpack8_bf16(z[1][q], b);
+          F2 g[4], s[4];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float s = logistic(a[k]);
-            o[0][k] = dv[k] * b[k] * s * (1.0f + a[k] * (1.0f - s));
-            o[1][k] = dv[k] * a[k] * s;
+          for (int k = 0; k < 4; ++k) g[k] = F2(a[2 * k], a[2 * k + 1]);
+          logistic_pairs<4>(g, s);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const F2 d2(dv[2 * k], dv[2 * k + 1]), gs = mul2(g[k], s[k]);
+            const F2 slope = fma2(gs, fma2(s[k], both(-1.0f), both(1.0f)), s[k]);
+            mul2(mul2(d2, F2(b[2 * k], b[2 * k + 1])), slope).get(o[0][2 * k], o[0][2 * k + 1]);
+            mul2(d2, gs).get(o[1][2 * k], o[1][2 * k + 1]);
           }
         } else {
-          float a[8] = {};
+          float a[8] = {}, s[8];
           if (kAct != MXB_ACT_NONE) unpack8_bf16(z[0][q], a);
+          slope8<kAct>(a, s);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) o[0][k] = dv[k] * act_slope<kAct>(a[k]);
+          for (int k = 0; k < 8; ++k) o[0][k] = dv[k] * s[k];
         }
 #pragma unroll
         for (int h = 0; h < kParts; ++h) {
@@ -105,7 +119,7 @@ __global__ void __launch_bounds__(kGradThreads) act_grad_kernel(const ActGradArg
             *reinterpret_cast<uint4*>(p.dz + (row * p.N + h * p.width + n) * 2) = pack8_bf16(o[h]);
         }
       }
-      if (p.codes) {
+      if constexpr (kQuant) {
 #pragma unroll
         for (int h = 0; h < kParts; ++h)
           quant_quad(p.codes, p.scales, o[h], in, row * p.N + h * p.width + n);
@@ -134,13 +148,13 @@ __global__ void __launch_bounds__(kGradThreads) act_grad_kernel(const ActGradArg
 // taking every eighth partial, added in warp order.
 __global__ void __launch_bounds__(kGradThreads) bias_sum_kernel(const float* __restrict__ partial,
                                                                 const int32_t* m_splits, int64_t M,
-                                                                int E, int N,
+                                                                int E, int N, int per,
                                                                 float* __restrict__ dbias) {
   __shared__ int32_t table[kGroupTableInts];
   __shared__ float red[kGradWarps][32];
   const GroupTable g{table, table + E + 1};
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp == 0) build_groups(g, m_splits, E, M, grad_chunks);
+  if (warp == 0) build_groups(g, m_splits, E, M, [&](int rows) { return grad_chunks(rows, per); });
   __syncthreads();
   const int e = blockIdx.y, n = blockIdx.x * 32 + lane;
   float s = 0.0f;
@@ -161,7 +175,10 @@ __global__ void __launch_bounds__(kGradThreads) bias_sum_kernel(const float* __r
 
 template <int kAct>
 void launch_act_grad(const ActGradArgs& p, int64_t blocks, int slabs, cudaStream_t s) {
-  act_grad_kernel<kAct><<<(unsigned)blocks, kGradThreads, 0, s>>>(p, slabs);
+  if (p.codes)
+    act_grad_kernel<kAct, true><<<(unsigned)blocks, kGradThreads, 0, s>>>(p, slabs);
+  else
+    act_grad_kernel<kAct, false><<<(unsigned)blocks, kGradThreads, 0, s>>>(p, slabs);
 }
 
 // ---------------------------------------------------------------- unpermute
@@ -186,7 +203,7 @@ struct UnpermuteMap {
   }
 };
 
-__global__ void __launch_bounds__(kUnpThreads) unpermute_kernel(const uint8_t* __restrict__ y,
+__global__ void __launch_bounds__(kUnpThreads, 4) unpermute_kernel(const uint8_t* __restrict__ y,
                                                                 const UnpermuteMap m, int64_t T,
                                                                 int64_t H,
                                                                 uint8_t* __restrict__ out) {
@@ -221,70 +238,62 @@ __global__ void __launch_bounds__(kUnpThreads) unpermute_kernel(const uint8_t* _
   }
 }
 
-// One CTA per token: dout's chunk is read once per eight rows, each row's dot
-// product is summed over lanes and warps in a fixed order.
-__global__ void __launch_bounds__(kUnpThreads) unpermute_grad_kernel(
+// A warp per (token, k): the row's dot product is one sum over the lanes, in a fixed
+// order, and the eight warps of a CTA read the same token's dout, mostly from L1.
+// (4096 tokens x 8 rows x 7168: 164 us; a CTA per token with eight rows a thread 265.)
+template <bool kQuant>
+__global__ void __launch_bounds__(kUnpThreads, kQuant ? 2 : 6) unpermute_grad_kernel(
     const uint8_t* __restrict__ dout, const uint8_t* __restrict__ y, const UnpermuteMap m,
     int64_t T, int64_t H, uint8_t* __restrict__ dy, uint8_t* __restrict__ codes,
     uint8_t* __restrict__ scales, float* __restrict__ dweight) {
-  __shared__ float red[kUnpThreads / 32][kUnpBatch];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t per_row = H / 8;
-  for (int64_t t = blockIdx.x; t < T; t += gridDim.x) {
-    for (int k0 = 0; k0 < m.topk; k0 += kUnpBatch) {
-      int64_t row[kUnpBatch];
-      float w[kUnpBatch], dot[kUnpBatch] = {};
+  constexpr int kUnroll = 2;
+  const int lane = threadIdx.x & 31;
+  const int64_t per_row = H / 8, items = T * m.topk;
+  for (int64_t i = (int64_t)blockIdx.x * (kUnpThreads / 32) + (threadIdx.x >> 5); i < items;
+       i += (int64_t)gridDim.x * (kUnpThreads / 32)) {
+    const int64_t t = i / m.topk;
+    const int k = (int)(i % m.topk);
+    const int64_t row = m.row(t, k);
+    if (row < 0) {
+      if (dweight && lane == 0) dweight[i] = 0.0f;
+      continue;
+    }
+    const float w = m.w(t, k);
+    const uint8_t* dt = dout + t * H * 2;
+    float dot = 0.0f;
+    for (int64_t c0 = 0; c0 < per_row; c0 += 32 * kUnroll) {
+      uint4 d[kUnroll], v[kUnroll];
 #pragma unroll
-      for (int k = 0; k < kUnpBatch; ++k) {
-        row[k] = k0 + k < m.topk ? m.row(t, k0 + k) : -1;
-        w[k] = row[k] >= 0 ? m.w(t, k0 + k) : 0.0f;
+      for (int u = 0; u < kUnroll; ++u) {
+        const int64_t c = c0 + 32 * u + lane;
+        if (c < per_row) {
+          d[u] = __ldg(reinterpret_cast<const uint4*>(dt + c * 16));
+          if (dweight) v[u] = ld_stream_v4(y + (row * H + c * 8) * 2);
+        }
       }
-      for (int64_t c0 = warp * 32; c0 < per_row; c0 += kUnpThreads) {  // the same for a warp
-        const int64_t c = c0 + lane;
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        if (c0 + 32 * u >= per_row) break;  // the same for the whole warp
+        const int64_t c = c0 + 32 * u + lane;
         const bool in = c < per_row;
-        uint4 d = make_uint4(0u, 0u, 0u, 0u), v[kUnpBatch];
-        if (in) d = *reinterpret_cast<const uint4*>(dout + (t * H + c * 8) * 2);
-        if (dweight) {
+        float dv[8] = {};
+        if (in) unpack8_bf16(d[u], dv);
+        if (dweight && in) {
+          float x[8];
+          unpack8_bf16(v[u], x);
 #pragma unroll
-          for (int k = 0; k < kUnpBatch; ++k)
-            if (in && row[k] >= 0) v[k] = ld_stream_v4(y + (row[k] * H + c * 8) * 2);
+          for (int j = 0; j < 8; ++j) dot += dv[j] * x[j];
         }
-        float dv[8];
-        unpack8_bf16(d, dv);
 #pragma unroll
-        for (int k = 0; k < kUnpBatch; ++k) {
-          if (row[k] < 0) continue;  // the same for the whole CTA
-          if (dweight && in) {
-            float x[8];
-            unpack8_bf16(v[k], x);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) dot[k] += dv[j] * x[j];
-          }
-          if (dy || codes) {
-            float o[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) o[j] = w[k] * dv[j];
-            if (dy && in)
-              *reinterpret_cast<uint4*>(dy + (row[k] * H + c * 8) * 2) = pack8_bf16(o);
-            if (codes) quant_quad(codes, scales, o, in, row[k] * H + c * 8);
-          }
-        }
+        for (int j = 0; j < 8; ++j) dv[j] *= w;
+        if (dy && in) *reinterpret_cast<uint4*>(dy + (row * H + c * 8) * 2) = pack8_bf16(dv);
+        if constexpr (kQuant) quant_quad(codes, scales, dv, in, row * H + c * 8);
       }
-      if (!dweight) continue;
+    }
+    if (dweight) {
 #pragma unroll
-      for (int k = 0; k < kUnpBatch; ++k) {
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) dot[k] += __shfl_xor_sync(0xffffffffu, dot[k], d);
-        if (lane == 0) red[warp][k] = dot[k];
-      }
-      __syncthreads();
-      if (threadIdx.x < kUnpBatch && k0 + (int)threadIdx.x < m.topk) {
-        float s = 0.0f;
-#pragma unroll
-        for (int q = 0; q < kUnpThreads / 32; ++q) s += red[q][threadIdx.x];
-        dweight[t * m.topk + k0 + threadIdx.x] = s;
-      }
-      __syncthreads();
+      for (int s = 16; s > 0; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
+      if (lane == 0) dweight[i] = dot;
     }
   }
 }
@@ -306,8 +315,9 @@ mxb_status check_unpermute(const char* what, int64_t R, int64_t H, int64_t map_p
 using namespace mxb;
 
 extern "C" int64_t mxb_bias_act_grad_workspace(int64_t M, int32_t E, int64_t N) {
-  if (M <= kGradRows || E < 1 || N < 1) return 0;
-  return most_grad_chunks(M, E) * N * 4;
+  const int per = grad_rows(M, N);
+  if (M <= per || E < 1 || N < 1) return 0;
+  return most_grad_chunks(M, E, per) * N * 4;
 }
 
 extern "C" mxb_status mxb_bias_act_grad(const void* dy, const void* pre, int64_t M,
@@ -354,12 +364,13 @@ extern "C" mxb_status mxb_bias_act_grad(const void* dy, const void* pre, int64_t
   p.E = E;
   p.N = (int)N;
   p.width = (int)(N / parts);
+  p.per = grad_rows(M, N);
   p.dz = (uint8_t*)dz;
   p.codes = (uint8_t*)dz_codes;
   p.scales = (uint8_t*)dz_scales;
   p.sums = !dbias ? nullptr : need ? (float*)workspace : dbias;
   const int slabs = (int)cdiv(p.width, kGradCols);
-  const int64_t blocks = (M <= kGradRows ? (int64_t)E : most_grad_chunks(M, E)) * slabs;
+  const int64_t blocks = (M <= p.per ? (int64_t)E : most_grad_chunks(M, E, p.per)) * slabs;
   MXB_REQUIRE(blocks <= INT32_MAX, MXB_ERR_INVALID_ARGUMENT, "%s: too many blocks", what);
   switch (activation) {
     case MXB_ACT_NONE: launch_act_grad<MXB_ACT_NONE>(p, blocks, slabs, s); break;
@@ -374,7 +385,7 @@ extern "C" mxb_status mxb_bias_act_grad(const void* dy, const void* pre, int64_t
     const mxb_status st = launch_status(what);
     if (st != MXB_OK) return st;
     bias_sum_kernel<<<dim3((unsigned)cdiv(N, 32), (unsigned)E), kGradThreads, 0, s>>>(
-        (const float*)workspace, m_splits, M, E, (int)N, dbias);
+        (const float*)workspace, m_splits, M, E, (int)N, p.per, dbias);
   }
   return launch_status(what);
 }
@@ -414,9 +425,9 @@ extern "C" mxb_status mxb_moe_unpermute_grad(const void* dout, const void* y, in
                   aligned(map, 4) && aligned(weight, 4) && aligned(dweight, 4),
               MXB_ERR_MISALIGNED, "%s: operands must be 16-byte aligned", what);
   const UnpermuteMap m{map, map_pitch, weight, topk, R};
-  unpermute_grad_kernel<<<(unsigned)std::min<int64_t>(T, INT32_MAX), kUnpThreads, 0,
-                          to_cuda(stream)>>>(
-      (const uint8_t*)dout, (const uint8_t*)y, m, T, H, (uint8_t*)dy, (uint8_t*)dy_codes,
-      (uint8_t*)dy_scales, dweight);
+  const auto kernel = dy_codes ? unpermute_grad_kernel<true> : unpermute_grad_kernel<false>;
+  kernel<<<(unsigned)std::min<int64_t>(cdiv(T * topk, kUnpThreads / 32), INT32_MAX), kUnpThreads, 0,
+           to_cuda(stream)>>>((const uint8_t*)dout, (const uint8_t*)y, m, T, H, (uint8_t*)dy,
+                              (uint8_t*)dy_codes, (uint8_t*)dy_scales, dweight);
   return launch_status(what);
 }

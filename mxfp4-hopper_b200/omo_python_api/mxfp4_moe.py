@@ -2,8 +2,8 @@
 a fused epilogue, their gradients, and the weighted way back to token order.
 
 No reference counterpart: the reference converts the permuted MXFP4 rows to FP8 and hands
-them to Transformer Engine's grouped GEMM.  Outputs are allocated here and filled by the
-sm_100a kernels through `omo`, on torch's current stream, without host synchronisation:
+them to Transformer Engine's grouped GEMM.  Outputs are allocated on the call and filled by
+the sm_100a kernels through `omo`, on torch's current stream, without host synchronisation:
 `m_splits` (rows per expert, in the order of the rows) stays on the device.
 """
 from __future__ import annotations
@@ -14,12 +14,11 @@ import torch
 
 import mxfp4_b200  # noqa: F401
 from mxfp4_b200.capi import ACTIVATIONS
-from omo import omo_bias_act_grad as _act_grad_op
-from omo import omo_bias_act_grad_workspace as _act_grad_workspace
-from omo import omo_grouped_gemm_mxfp4 as _gemm_op
+from omo import omo_bias_act_grad_new as _act_grad_op
+from omo import omo_grouped_gemm_mxfp4_new as _gemm_op
 from omo import omo_grouped_wgrad_mxfp4 as _wgrad_op
-from omo import omo_moe_unpermute as _unpermute_op
-from omo import omo_moe_unpermute_grad as _unpermute_grad_op
+from omo import omo_moe_unpermute_grad_new as _unpermute_grad_op
+from omo import omo_moe_unpermute_new as _unpermute_op
 from omo import omo_swizzle_scales_grouped as _swizzle_op
 
 uint8_type = torch.uint8
@@ -61,17 +60,9 @@ def omo_grouped_gemm_mxfp4(a_codes: torch.Tensor, a_scales: torch.Tensor, b_code
     activation [M, N] (`save_pre`) and the result's rowwise MXFP4, codes [M, W/2] and scales
     [M, W/32] (`quantize`); `bf16_out=False` leaves the BF16 result out.  Rows past the sum
     of m_splits are not written."""
-    act = _activation(activation)
-    M, N = a_codes.shape[0], b_codes.shape[1]
-    W = N // 2 if activation == "swiglu" else N
-    dev = a_codes.device
-    c = torch.empty((M, W), device=dev, dtype=torch.bfloat16) if bf16_out else None
-    pre = torch.empty((M, N), device=dev, dtype=torch.bfloat16) if save_pre else None
-    q = torch.empty((M, W // 2), device=dev, dtype=uint8_type) if quantize else None
-    s = torch.empty((M, W // 32), device=dev, dtype=uint8_type) if quantize else None
-    _gemm_op(a_codes, a_scales, m_splits, b_codes, b_scales, c, bias, act, residual, pre, q, s)
-    out = tuple(x for x in (c, pre, q, s) if x is not None)
-    return out[0] if len(out) == 1 else out
+    out = _gemm_op(a_codes, a_scales, m_splits, b_codes, b_scales, bias, _activation(activation),
+                   residual, save_pre, quantize, bf16_out)
+    return out[0] if len(out) == 1 else tuple(out)
 
 
 def omo_gemm_mxfp4_act(a_codes: torch.Tensor, a_scales: torch.Tensor, b_codes: torch.Tensor,
@@ -81,8 +72,7 @@ def omo_gemm_mxfp4_act(a_codes: torch.Tensor, a_scales: torch.Tensor, b_codes: t
     """One dense layer: act(A . B^T + bias) + residual with b_codes [N, K/2], b_scales [its
     128x4-tile rows, ...] and bias [N]; otherwise as `omo_grouped_gemm_mxfp4`.  Any number of
     rows, N % 8 == 0 (swiglu: N % 16 == 0), K % 32 == 0."""
-    return omo_grouped_gemm_mxfp4(a_codes, a_scales, b_codes.unsqueeze(0), b_scales.unsqueeze(0),
-                                  None, None if bias is None else bias.unsqueeze(0), activation,
+    return omo_grouped_gemm_mxfp4(a_codes, a_scales, b_codes, b_scales, None, bias, activation,
                                   residual, save_pre, quantize, bf16_out)
 
 
@@ -109,24 +99,8 @@ def omo_bias_act_grad(dy: torch.Tensor, pre: Optional[torch.Tensor],
     FP32 = the sum of dz over every expert's rows.  Returns (dz, dbias, codes, scales) without
     what was not asked for; codes [M, N/2] and scales [M, N/32] (`quantize`) are the rowwise
     MXFP4 of dz, the left operand of the input gradient's product."""
-    act = _activation(activation)
-    if pre is None and activation != "none":
-        raise RuntimeError("pre is needed for this activation")
-    M = dy.shape[0]
-    N = dy.shape[1] * 2 if activation == "swiglu" else dy.shape[1]
-    E = 1 if m_splits is None else m_splits.shape[0]
-    dev = dy.device
-    dz = torch.empty((M, N), device=dev, dtype=torch.bfloat16) if bf16_out else None
-    q = torch.empty((M, N // 2), device=dev, dtype=uint8_type) if quantize else None
-    s = torch.empty((M, N // 32), device=dev, dtype=uint8_type) if quantize else None
-    db = work = None
-    if bias_grad:
-        db = torch.empty((E, N), device=dev, dtype=torch.float32)
-        nbytes = _act_grad_workspace(M, E, N)
-        work = torch.empty(nbytes, device=dev, dtype=uint8_type) if nbytes else None
-    _act_grad_op(dy, pre, m_splits, E, N, act, dz, q, s, db, work)
-    out = tuple(x for x in (dz, db, q, s) if x is not None)
-    return out[0] if len(out) == 1 else out
+    out = _act_grad_op(dy, pre, m_splits, _activation(activation), bias_grad, quantize, bf16_out)
+    return out[0] if len(out) == 1 else tuple(out)
 
 
 def omo_moe_unpermute(y: torch.Tensor, row_map: torch.Tensor,
@@ -136,10 +110,7 @@ def omo_moe_unpermute(y: torch.Tensor, row_map: torch.Tensor,
     `omo_moe_permute_mxfp4` with its `dst` (negative or too large: no row).  y BF16 [R, H],
     row_map int32 [T, topk], weight FP32 [T, topk] or None (ones); `topk` takes the first
     columns of a wider map (a row_id_map: topk = E)."""
-    k = row_map.shape[1] if topk is None else topk
-    out = torch.empty((row_map.shape[0], y.shape[1]), device=y.device, dtype=torch.bfloat16)
-    _unpermute_op(y, row_map, weight, k, out)
-    return out
+    return _unpermute_op(y, row_map, weight, row_map.shape[1] if topk is None else topk)
 
 
 def omo_moe_unpermute_grad(dout: torch.Tensor, y: torch.Tensor, row_map: torch.Tensor,
@@ -151,14 +122,6 @@ def omo_moe_unpermute_grad(dout: torch.Tensor, y: torch.Tensor, row_map: torch.T
     Returns (dy, dweight, codes, scales) without what was not asked for; codes and scales
     (`quantize`) are dy's rowwise MXFP4.  Rows that row_map does not name are left
     uninitialised, or zero with `zero_unnamed`."""
-    k = row_map.shape[1] if topk is None else topk
-    R, H = y.shape
-    dev = y.device
-    new = torch.zeros if zero_unnamed else torch.empty
-    dy = new((R, H), device=dev, dtype=torch.bfloat16)
-    q = new((R, H // 2), device=dev, dtype=uint8_type) if quantize else None
-    s = new((R, H // 32), device=dev, dtype=uint8_type) if quantize else None
-    dw = torch.empty((row_map.shape[0], k), device=dev, dtype=torch.float32) if weight_grad else None
-    _unpermute_grad_op(dout, y, R, row_map, weight, k, dy, q, s, dw)
-    out = tuple(x for x in (dy, dw, q, s) if x is not None)
-    return out[0] if len(out) == 1 else out
+    out = _unpermute_grad_op(dout, y, row_map, weight, row_map.shape[1] if topk is None else topk,
+                             weight_grad, quantize, zero_unnamed)
+    return out[0] if len(out) == 1 else tuple(out)

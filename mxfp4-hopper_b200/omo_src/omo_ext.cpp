@@ -495,28 +495,34 @@ void omo_swizzle_scales_grouped(at::Tensor scales, int64_t parts, at::Tensor out
                "omo_swizzle_scales_grouped");
 }
 
-void omo_grouped_gemm_mxfp4(at::Tensor a_codes, at::Tensor a_scales, OptTensor m_splits,
-                            at::Tensor b_codes, at::Tensor b_scales, OptTensor c, OptTensor bias,
-                            int64_t activation, OptTensor residual, OptTensor pre,
-                            OptTensor c_codes, OptTensor c_scales) {
+// b_codes [E, N, K/2], or [N, K/2] for a dense layer (then b_scales and bias lack the
+// leading dimension too).
+void omo_grouped_gemm_mxfp4(const at::Tensor& a_codes, const at::Tensor& a_scales,
+                            const OptTensor& m_splits, const at::Tensor& b_codes,
+                            const at::Tensor& b_scales, const OptTensor& c, const OptTensor& bias,
+                            int64_t activation, const OptTensor& residual, const OptTensor& pre,
+                            const OptTensor& c_codes, const OptTensor& c_scales) {
   OmoRange nvtx_range("omo_grouped_gemm_mxfp4");
   OMO_CHECK_INPUT(b_codes);
   check_dtype(b_codes, at::kByte, "b_codes");
-  TORCH_CHECK(b_codes.dim() == 3, "b_codes must be [E, N, K/2]");
+  const bool dense = b_codes.dim() == 2;
+  TORCH_CHECK(dense || b_codes.dim() == 3, "b_codes must be [E, N, K/2] or [N, K/2]");
   TORCH_CHECK(a_codes.dim() == 2, "a_codes must be [M, K/2]");
   TORCH_CHECK(activation >= MXB_ACT_NONE && activation <= MXB_ACT_SWIGLU, "unknown activation");
-  const int64_t E = b_codes.size(0), N = b_codes.size(1), K = b_codes.size(2) * 2;
+  const int64_t E = dense ? 1 : b_codes.size(0), N = b_codes.size(-2), K = b_codes.size(-1) * 2;
   const int64_t M = a_codes.size(0), parts = activation == MXB_ACT_SWIGLU ? 2 : 1, W = N / parts;
   TORCH_CHECK(E >= 1 && N % parts == 0 && K % 32 == 0, "b_codes must be [E, N, K/2] with K % 32 == 0");
   check_rows(a_codes, "a_codes", M, K / 2, at::kByte, b_codes);
   check_rows(a_scales, "a_scales", M, K / 32, at::kByte, b_codes);
-  check_dense(b_scales, "b_scales", {E, parts * ((W + 127) / 128 * 128), (K / 32 + 3) / 4 * 4},
-              at::kByte, b_codes);
+  const int64_t tiled[3] = {E, parts * ((W + 127) / 128 * 128), (K / 32 + 3) / 4 * 4};
+  check_dense(b_scales, "b_scales", at::IntArrayRef(tiled + dense, 3 - dense), at::kByte, b_codes);
   mxb_epilogue ep = {};
   ep.activation = (int32_t)activation;
   if (bias) {
     ep.bias_f32 = bias->scalar_type() == at::kFloat;
-    check_dense(*bias, "bias", {E, N}, ep.bias_f32 ? at::kFloat : at::kBFloat16, b_codes);
+    const int64_t each[2] = {E, N};
+    check_dense(*bias, "bias", at::IntArrayRef(each + dense, 2 - dense),
+                ep.bias_f32 ? at::kFloat : at::kBFloat16, b_codes);
     ep.bias = bias->data_ptr();
   }
   if (residual) {
@@ -547,6 +553,31 @@ void omo_grouped_gemm_mxfp4(at::Tensor a_codes, at::Tensor a_scales, OptTensor m
                                       pitch(a_scales), M, splits, (int32_t)E, b_codes.data_ptr(),
                                       b_scales.data_ptr(), N, K, &ep, opt_ptr(c), cur_stream()),
                "omo_grouped_gemm_mxfp4");
+}
+
+// The same with the results allocated here (a call from Python that allocates them
+// one by one costs several microseconds more, as much as a decoding step's kernel):
+// returns those of (c, pre, c_codes, c_scales) that are asked for.
+std::vector<at::Tensor> omo_grouped_gemm_mxfp4_new(
+    const at::Tensor& a_codes, const at::Tensor& a_scales, const OptTensor& m_splits,
+    const at::Tensor& b_codes, const at::Tensor& b_scales, const OptTensor& bias,
+    int64_t activation, const OptTensor& residual, bool save_pre, bool quantize, bool bf16_out) {
+  TORCH_CHECK(a_codes.dim() == 2 && b_codes.dim() >= 2, "a_codes [M, K/2], b_codes [.., N, K/2]");
+  TORCH_CHECK(bf16_out || save_pre || quantize, "no result is asked for");
+  const int64_t M = a_codes.size(0), N = b_codes.size(-2);
+  const int64_t W = activation == MXB_ACT_SWIGLU ? N / 2 : N;
+  const auto bf16 = a_codes.options().dtype(at::kBFloat16);
+  OptTensor c, pre, q, s;
+  std::vector<at::Tensor> out;
+  if (bf16_out) out.push_back(*(c = at::empty({M, W}, bf16)));
+  if (save_pre) out.push_back(*(pre = at::empty({M, N}, bf16)));
+  if (quantize) {
+    out.push_back(*(q = at::empty({M, W / 2}, a_codes.options())));
+    out.push_back(*(s = at::empty({M, W / 32}, a_codes.options())));
+  }
+  omo_grouped_gemm_mxfp4(a_codes, a_scales, m_splits, b_codes, b_scales, c, bias, activation,
+                         residual, pre, q, s);
+  return out;
 }
 
 void omo_grouped_wgrad_mxfp4(at::Tensor dy, at::Tensor x_codes, at::Tensor x_scales,
@@ -610,6 +641,31 @@ void omo_bias_act_grad(at::Tensor dy, OptTensor pre, OptTensor m_splits, int64_t
       "omo_bias_act_grad");
 }
 
+// The same with results and workspace allocated here: those of (dz, dbias, dz_codes,
+// dz_scales) that are asked for.
+std::vector<at::Tensor> omo_bias_act_grad_new(const at::Tensor& dy, const OptTensor& pre,
+                                              const OptTensor& m_splits, int64_t activation,
+                                              bool bias_grad, bool quantize, bool bf16_out) {
+  TORCH_CHECK(dy.is_cuda() && dy.dim() == 2, "dy must be a CUDA tensor [M, W]");
+  const int64_t M = dy.size(0), N = dy.size(1) * (activation == MXB_ACT_SWIGLU ? 2 : 1);
+  const int64_t E = m_splits ? m_splits->numel() : 1;
+  const auto bytes = dy.options().dtype(at::kByte);
+  OptTensor dz, db, q, s, work;
+  std::vector<at::Tensor> out;
+  if (bf16_out) out.push_back(*(dz = at::empty({M, N}, dy.options().dtype(at::kBFloat16))));
+  if (bias_grad) {
+    out.push_back(*(db = at::empty({E, N}, dy.options().dtype(at::kFloat))));
+    const int64_t need = mxb_bias_act_grad_workspace(M, (int32_t)E, N);
+    if (need) work = at::empty({need}, bytes);
+  }
+  if (quantize) {
+    out.push_back(*(q = at::empty({M, N / 2}, bytes)));
+    out.push_back(*(s = at::empty({M, N / 32}, bytes)));
+  }
+  omo_bias_act_grad(dy, pre, m_splits, E, N, activation, dz, q, s, db, work);
+  return out;
+}
+
 // map int32 [T, >= topk] (row pitch = its stride); topk from the weights, or all columns.
 int64_t check_map(const at::Tensor& map, const OptTensor& weight, int64_t topk,
                   const at::Tensor& like) {
@@ -660,6 +716,39 @@ void omo_moe_unpermute_grad(at::Tensor dout, OptTensor y, int64_t rows, at::Tens
                                       opt_ptr(dy_codes), opt_ptr(dy_scales),
                                       (float*)opt_ptr(dweight), cur_stream()),
                "omo_moe_unpermute_grad");
+}
+
+at::Tensor omo_moe_unpermute_new(const at::Tensor& y, const at::Tensor& map,
+                                 const OptTensor& weight, int64_t topk) {
+  TORCH_CHECK(y.is_cuda() && y.dim() == 2 && map.dim() == 2, "y must be a CUDA tensor [R, H], map [T, k]");
+  at::Tensor out = at::empty({map.size(0), y.size(1)}, y.options());
+  omo_moe_unpermute(y, map, weight, topk, out);
+  return out;
+}
+
+// Those of (dy, dweight, dy_codes, dy_scales) that are asked for; zero: rows that the map
+// does not name are zero instead of uninitialised.
+std::vector<at::Tensor> omo_moe_unpermute_grad_new(const at::Tensor& dout, const at::Tensor& y,
+                                                   const at::Tensor& map, const OptTensor& weight,
+                                                   int64_t topk, bool weight_grad, bool quantize,
+                                                   bool zero) {
+  TORCH_CHECK(y.is_cuda() && y.dim() == 2 && map.dim() == 2, "y must be a CUDA tensor [R, H], map [T, k]");
+  const int64_t R = y.size(0), H = y.size(1);
+  const auto bytes = y.options().dtype(at::kByte);
+  auto make = [&](at::IntArrayRef sizes, const at::TensorOptions& o) {
+    return zero ? at::zeros(sizes, o) : at::empty(sizes, o);
+  };
+  c10::cuda::CUDAGuard g(y.device());
+  at::Tensor dy = make({R, H}, y.options());
+  OptTensor dw, q, s;
+  std::vector<at::Tensor> out = {dy};
+  if (weight_grad) out.push_back(*(dw = at::empty({map.size(0), topk}, y.options().dtype(at::kFloat))));
+  if (quantize) {
+    out.push_back(*(q = make({R, H / 2}, bytes)));
+    out.push_back(*(s = make({R, H / 32}, bytes)));
+  }
+  omo_moe_unpermute_grad(dout, y, R, map, weight, topk, dy, q, s, dw);
+  return out;
 }
 
 }  // namespace
@@ -729,6 +818,15 @@ PYBIND11_MODULE(omo, m) {
         py::arg("b_scales"), py::arg("c"), py::arg("bias") = py::none(),
         py::arg("activation") = 0, py::arg("residual") = py::none(), py::arg("pre") = py::none(),
         py::arg("c_codes") = py::none(), py::arg("c_scales") = py::none());
+  m.def("omo_grouped_gemm_mxfp4_new", &omo_grouped_gemm_mxfp4_new,
+        "omo_grouped_gemm_mxfp4 with its results allocated", py::arg("a_codes"),
+        py::arg("a_scales"), py::arg("m_splits"), py::arg("b_codes"), py::arg("b_scales"),
+        py::arg("bias"), py::arg("activation"), py::arg("residual"), py::arg("save_pre"),
+        py::arg("quantize"), py::arg("bf16_out"));
+  m.def("omo_bias_act_grad_new", &omo_bias_act_grad_new,
+        "omo_bias_act_grad with its results allocated", py::arg("dy"), py::arg("pre"),
+        py::arg("m_splits"), py::arg("activation"), py::arg("bias_grad"), py::arg("quantize"),
+        py::arg("bf16_out"));
   m.def("omo_grouped_wgrad_mxfp4", &omo_grouped_wgrad_mxfp4,
         "Weight gradients grouped by expert from BF16 dy and MXFP4 x (tcgen05)", py::arg("dy"),
         py::arg("x_codes"), py::arg("x_scales"), py::arg("m_splits"), py::arg("dw"),
@@ -742,6 +840,13 @@ PYBIND11_MODULE(omo, m) {
         py::arg("workspace") = py::none());
   m.def("omo_moe_unpermute", &omo_moe_unpermute, "Weighted sum of expert rows per token",
         py::arg("y"), py::arg("map"), py::arg("weight"), py::arg("topk"), py::arg("out"));
+  m.def("omo_moe_unpermute_new", &omo_moe_unpermute_new,
+        "omo_moe_unpermute with its result allocated", py::arg("y"), py::arg("map"),
+        py::arg("weight"), py::arg("topk"));
+  m.def("omo_moe_unpermute_grad_new", &omo_moe_unpermute_grad_new,
+        "omo_moe_unpermute_grad with its results allocated", py::arg("dout"), py::arg("y"),
+        py::arg("map"), py::arg("weight"), py::arg("topk"), py::arg("weight_grad"),
+        py::arg("quantize"), py::arg("zero"));
   m.def("omo_moe_unpermute_grad", &omo_moe_unpermute_grad, "Gradient of omo_moe_unpermute",
         py::arg("dout"), py::arg("y"), py::arg("rows"), py::arg("map"), py::arg("weight"),
         py::arg("topk"), py::arg("dy") = py::none(), py::arg("dy_codes") = py::none(),

@@ -390,8 +390,10 @@ def test_act_grad_rows_of_nobody(cuda):
     dz = torch.full_like(pre, 5.0)
     db = torch.empty(2, 64, dtype=torch.float32, device=cuda)
     m = dev([10, -3])
+    need = capi.load().mxb_bias_act_grad_workspace(50, 2, 64)
+    work = torch.empty(need, dtype=torch.uint8, device=cuda)
     capi.call("mxb_bias_act_grad", dy.data_ptr(), pre.data_ptr(), 50, m.data_ptr(), 2, 64, 3,
-              dz.data_ptr(), None, None, db.data_ptr(), None, 0, H.stream())
+              dz.data_ptr(), None, None, db.data_ptr(), work.data_ptr(), need, H.stream())
     assert (dz[10:] == 5).all() and (db[1] == 0).all()
 
 
