@@ -329,7 +329,7 @@ extern "C" mxb_status mxb_bias_act_grad(const void* dy, const void* pre, int64_t
   MXB_REQUIRE(activation >= MXB_ACT_NONE && activation <= MXB_ACT_SWIGLU, MXB_ERR_INVALID_ARGUMENT,
               "%s: unknown activation %d", what, activation);
   const int parts = activation == MXB_ACT_SWIGLU ? 2 : 1;
-  MXB_REQUIRE(M >= 0 && M <= INT32_MAX && E >= 1 && E <= MXB_MAX_EXPERTS, MXB_ERR_INVALID_ARGUMENT,
+  MXB_REQUIRE(M >= 0 && M <= INT32_MAX - 512 && E >= 1 && E <= MXB_MAX_EXPERTS, MXB_ERR_INVALID_ARGUMENT,
               "%s: need 0 <= M < 2^31 and 1 <= E <= %d (M=%lld E=%d)", what, MXB_MAX_EXPERTS,
               (long long)M, E);
   MXB_REQUIRE(N >= 0 && N <= INT32_MAX - 512 && N % (8 * parts) == 0, MXB_ERR_INVALID_ARGUMENT,

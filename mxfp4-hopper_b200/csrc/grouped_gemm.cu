@@ -984,7 +984,7 @@ extern "C" mxb_status mxb_grouped_gemm_mxfp4(const void* a_codes, int64_t a_code
               MXB_ERR_INVALID_ARGUMENT, "%s: unknown activation %d", what, ep->activation);
   const bool glu = ep->activation == MXB_ACT_SWIGLU;
   const int64_t parts = glu ? 2 : 1;
-  MXB_REQUIRE(M >= 0 && M <= INT32_MAX && E >= 1 && E <= MXB_MAX_EXPERTS, MXB_ERR_INVALID_ARGUMENT,
+  MXB_REQUIRE(M >= 0 && M <= INT32_MAX - 512 && E >= 1 && E <= MXB_MAX_EXPERTS, MXB_ERR_INVALID_ARGUMENT,
               "%s: need 0 <= M < 2^31 and 1 <= E <= %d (M=%lld E=%d)", what, MXB_MAX_EXPERTS,
               (long long)M, E);
   MXB_REQUIRE(N >= 0 && N % (8 * parts) == 0 && K >= 32 && K % 32 == 0 && K <= (1 << 24),

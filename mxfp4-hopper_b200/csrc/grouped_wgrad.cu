@@ -384,7 +384,7 @@ extern "C" mxb_status mxb_grouped_wgrad_mxfp4(const void* dy, int64_t dy_ld, con
                                               int64_t K, void* dw, int32_t dw_f32,
                                               int32_t accumulate, mxb_stream_t stream) {
   const char* const what = "grouped_wgrad_mxfp4";
-  MXB_REQUIRE(M >= 0 && M <= INT32_MAX && E >= 1 && E <= MXB_MAX_EXPERTS, MXB_ERR_INVALID_ARGUMENT,
+  MXB_REQUIRE(M >= 0 && M <= INT32_MAX - 512 && E >= 1 && E <= MXB_MAX_EXPERTS, MXB_ERR_INVALID_ARGUMENT,
               "%s: need 0 <= M < 2^31 and 1 <= E <= %d (M=%lld E=%d)", what, MXB_MAX_EXPERTS,
               (long long)M, E);
   MXB_REQUIRE(N >= 0 && N <= INT32_MAX - 512 && N % 8 == 0 && K >= 0 && K <= INT32_MAX - 512 &&

@@ -89,8 +89,9 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
 
 // mbar_wait() that lets the hardware suspend the thread for up to kSuspendNs a
 // round instead of polling, so that waiting warps leave the issue slots to the
-// others.  kSuspendRounds bound the wait at a second or so.
-constexpr uint32_t kSuspendNs = 10000, kSuspendRounds = 1u << 17;
+// others.  kSuspendRounds bound the wait at about a minute, and at the better part
+// of a second if no round is suspended (a tile of 2^24 columns of K takes 20 ms).
+constexpr uint32_t kSuspendNs = 2000, kSuspendRounds = 1u << 25;
 __device__ __forceinline__ bool mbar_wait_suspend(uint64_t* bar, uint32_t parity) {
   const uint32_t a = smem_addr(bar);
   for (uint32_t i = 0; i < kSuspendRounds; ++i) {

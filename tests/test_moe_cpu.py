@@ -113,3 +113,13 @@ def test_workspace_size():
     assert f(32, 8, 4096) == 0           # one block of rows per expert: no partial sums
     assert f(33, 8, 4096) == 9 * 4096 * 4
     assert f(16384, 8, 4096) == (128 + 8) * 4096 * 4
+
+
+def test_expert_order():
+    """Rows sorted by expert, tokens in order within an expert; empty experts have no rows."""
+    import torch
+    from mxfp4_b200.moe import expert_order
+    idx = torch.tensor([[2, 0], [0, 3], [2, 3], [3, 0]])
+    dst, splits = expert_order(idx, 5)
+    assert splits.tolist() == [3, 0, 2, 3, 0] and splits.dtype == torch.int32
+    assert dst.tolist() == [[3, 0], [1, 5], [4, 6], [7, 2]] and dst.dtype == torch.int32
