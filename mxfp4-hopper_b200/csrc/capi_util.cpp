@@ -108,4 +108,26 @@ bool make_tensor_map_2d(CUtensorMap* map, const void* base, CUtensorMapDataType 
   return true;
 }
 
+bool make_tensor_map_3d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype,
+                        int elem_bytes, int64_t planes, int64_t rows, int64_t cols,
+                        uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+  auto fn = encode_fn();
+  if (!fn) {
+    set_error("cuTensorMapEncodeTiled is unavailable from the driver");
+    return false;
+  }
+  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+  cuuint64_t strides[2] = {(cuuint64_t)(cols * elem_bytes), (cuuint64_t)(rows * cols * elem_bytes)};
+  cuuint32_t box[3] = {box_cols, box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, dtype, 3, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
+    return false;
+  }
+  return true;
+}
+
 }  // namespace mxb

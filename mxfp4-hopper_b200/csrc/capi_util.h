@@ -50,6 +50,12 @@ bool make_tensor_map_2d(CUtensorMap* map, const void* base, CUtensorMapDataType 
                         uint32_t box_rows,
                         CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_NONE);
 
+// Host: the same over contiguous [planes, rows, cols] with a box of one plane: what
+// lies past a plane's rows is not reached.
+bool make_tensor_map_3d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype,
+                        int elem_bytes, int64_t planes, int64_t rows, int64_t cols,
+                        uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle);
+
 // Registry of per-translation-unit wait-timeout counters (see tma.cuh).
 // Returns true so that it can initialise a namespace-scope constant.
 bool register_wait_timeout_reader(unsigned int (*reader)(bool reset));

@@ -158,6 +158,27 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int32_t x, 
       "r"(x), "r"(y), "r"(smem_addr(src))
       : "memory");
 }
+// A box of a 3-D tensor, written or (kAdd, f32) added to global memory, from a warp
+// that runs converged: issued by the lane with `one` true, so that the operands stay
+// in uniform registers (from a single-lane branch a store took about 700 cycles to issue).
+template <bool kAdd>
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, int32_t x, int32_t y,
+                                             int32_t z, const void* src, bool one) {
+  if constexpr (kAdd)
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.b32 q, %5, 0;\n"
+        " @q cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group"
+        " [%0, {%1, %2, %3}], [%4];\n}" ::"l"(reinterpret_cast<uint64_t>(map)),
+        "r"(x), "r"(y), "r"(z), "r"(smem_addr(src)), "r"((uint32_t)one)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.b32 q, %5, 0;\n"
+        " @q cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group"
+        " [%0, {%1, %2, %3}], [%4];\n}" ::"l"(reinterpret_cast<uint64_t>(map)),
+        "r"(x), "r"(y), "r"(z), "r"(smem_addr(src)), "r"((uint32_t)one)
+        : "memory");
+}
 // 1-D bulk copy of `bytes` contiguous bytes shared -> global (bulk group).
 // Both addresses 16-byte aligned, bytes a multiple of 16.
 __device__ __forceinline__ void bulk_store_1d(void* dst, const void* src, uint32_t bytes) {
