@@ -13,7 +13,7 @@
 // epilogue then has 32 rows of dw and writes (or adds) them 128 bytes of a row at a
 // time by TMA from a staging box of its own: whole lines, clipped to the expert.
 // (With rows as columns of the accumulator a BF16 dw left in 64-byte pieces: 1650 us
-// instead of STORE_US for 32 experts of 4096 x 7168 with 4096 rows.)
+// instead of 490 for 32 experts of 4096 x 7168 with 4096 rows.)
 //
 // Ragged groups: a step's rows past its expert's end are expanded as zeros, and
 // the same rows of dy (the next expert's, whatever they hold) are overwritten
@@ -34,12 +34,12 @@ namespace mxb {
 namespace {
 
 constexpr int kWgThreads = 448;  // TMA, MMA, 4 epilogue warps, 8 expanding warps
-constexpr int kWgStages = 6;
+constexpr int kWgStages = 5;
 constexpr int kWgRows = 64;                 // rows per step
 constexpr int kTileX = 256, kTileY = 256;   // columns of x and of dy, half in each CTA
 constexpr uint32_t kWgBox = kWgRows * 128;  // 64 rows x 64 bf16 columns
 constexpr uint32_t kWgX = 2 * kWgBox, kWgStage = 2 * kWgX;
-constexpr uint32_t kWgOut = 32 * 128;       // staging of an epilogue warp: 32 rows of 128 bytes
+constexpr uint32_t kWgOut = 2 * 32 * 128;   // two boxes of an epilogue warp: 32 rows of 128 bytes
 constexpr size_t kWgSmem = 1024 + kWgStages * kWgStage + 4 * kWgOut + kGroupTableInts * 4 + 256;
 static_assert(kWgSmem <= 227 * 1024, "one CTA per SM");
 
@@ -220,7 +220,8 @@ __global__ void __launch_bounds__(kWgThreads, 1) grouped_wgrad_kernel(
     // ------------------------------------------------ epilogue: lane = column of dy
     const int quad = warp & 3;
     const uint32_t acc_empty0 = peer_addr(smem_addr(acc_empty), 0);
-    uint8_t* box = staging + quad * kWgOut;
+    uint8_t* boxes = staging + quad * kWgOut;
+    int turn = 0;
     constexpr int kCols = kF32 ? 32 : 64;  // 128 bytes of a row
     for (int i = 0; i < my_tiles; ++i) {
       const Tile tl = tile_at(i);
@@ -249,8 +250,10 @@ __global__ void __launch_bounds__(kWgThreads, 1) grouped_wgrad_kernel(
 #pragma unroll
           for (int j = 0; j < 32; ++j) w[j] = 0u;
         }
-        bulk_wait_read_all();  // the box's last store has read it
+        bulk_wait_read_1();  // the store before the last, of this box, has read it
         __syncwarp();
+        uint8_t* box = boxes + turn * (kWgOut / 2);
+        turn ^= 1;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           *reinterpret_cast<uint4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) =
