@@ -174,8 +174,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
     const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ GroupedArgs p) {
   constexpr bool kGlu = kAct == MXB_ACT_SWIGLU;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                             ~uintptr_t(1023));
+  uint8_t* smem = align_1024(smem_raw);
   uint8_t* scales = smem + kWideStages * kWideStage;
   float* bias_s = reinterpret_cast<float*>(scales + kSbStages * kSbStage);
   // CTA 0's: a step's codes of both CTAs have landed and its scales are in tensor memory
@@ -564,8 +563,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) grouped_narrow_kernel(
   using L = Narrow<kGlu, kT>;
   constexpr int kBlocks = L::kBlocks, kStages = L::kStages;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                             ~uintptr_t(1023));
+  uint8_t* smem = align_1024(smem_raw);
   float* part = reinterpret_cast<float*>(smem + kStages * L::kStage);
   uint8_t* row_bytes = reinterpret_cast<uint8_t*>(part + L::kPart / 4);  // 1 KB a scale warp
   uint64_t* full = reinterpret_cast<uint64_t*>(row_bytes + 2 * 1024);

@@ -92,8 +92,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) grouped_wgrad_kernel(
     const __grid_constant__ CUtensorMap map_dy, const __grid_constant__ CUtensorMap map_dw,
     const __grid_constant__ WgradArgs p) {
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                             ~uintptr_t(1023));
+  uint8_t* smem = align_1024(smem_raw);
   uint8_t* staging = smem + kWgStages * kWgStage;
   uint64_t* dy_full = reinterpret_cast<uint64_t*>(staging + 4 * kWgOut);
   uint64_t* full = dy_full + kWgStages;  // CTA 0's: both CTAs' halves are in place
