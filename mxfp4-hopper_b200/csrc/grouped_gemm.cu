@@ -196,7 +196,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
   const int ksteps = (p.K + kStepK - 1) / kStepK;
   const int S = p.K / 32, S4 = (S + 3) / 4;
 
+  allow_next_kernel();
   if (warp == 0) {
+    wait_for_previous_kernel();
     build_groups(g, p.m_splits, p.E, p.M, [&](int rows) { return (rows + 255) / 256 * ntn; });
   } else if (warp == 1) {
     tmem_alloc_pair(tmem_slot, kTmemCols);
@@ -218,6 +220,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
   __syncthreads();
   tc_fence_after();
   cluster_sync();
+  wait_for_previous_kernel();
   const uint32_t tmem = *tmem_slot;
   const int tiles = g.tile[p.E];
   const int pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;
@@ -585,7 +588,9 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) grouped_narrow_kernel(
   const int k_end = (int)((int64_t)ksteps * (rank + 1) / ranks);
   const int S = p.K / 32, S4 = (S + 3) / 4;
 
+  allow_next_kernel();
   if (warp == 0) {
+    wait_for_previous_kernel();
     build_groups(g, p.m_splits, p.E, p.M, [&](int rows) { return (rows + kT - 1) / kT * ntn; });
   } else if (warp == 1) {
     tmem_alloc(tmem_slot, kTmemCols);
@@ -608,6 +613,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) grouped_narrow_kernel(
   __syncthreads();
   tc_fence_after();
   cluster_sync();  // every CTA's barriers are ready for its peers
+  wait_for_previous_kernel();
   const uint32_t tmem = *tmem_slot;
   const int tiles = g.tile[p.E];
   const int cluster = (int)(blockIdx.x / ranks), clusters = (int)(gridDim.x / ranks);

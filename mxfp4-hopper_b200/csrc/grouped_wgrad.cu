@@ -109,7 +109,9 @@ __global__ void __launch_bounds__(kWgThreads, 1) grouped_wgrad_kernel(
   const int per_expert = nty * ntx;
   const int rank = (int)cluster_rank();
 
+  allow_next_kernel();
   if (warp == 0) {
+    wait_for_previous_kernel();
     build_groups(g, p.m_splits, p.E, p.M, [&](int) { return 0; });
   } else if (warp == 1) {
     tmem_alloc_pair(tmem_slot, 512);
@@ -130,6 +132,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) grouped_wgrad_kernel(
   __syncthreads();
   tc_fence_after();
   cluster_sync();
+  wait_for_previous_kernel();
   const uint32_t tmem = *tmem_slot;
   const int tiles = p.E * per_expert;
   const int pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;

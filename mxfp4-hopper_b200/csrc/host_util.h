@@ -36,7 +36,9 @@ inline int sm_count() {
   return n;
 }
 
-// Launches `clusters` clusters of `size` CTAs.
+// Launches `clusters` clusters of `size` CTAs.  The kernel may start while the one
+// before it in the stream is finishing (it sets up its barriers and tensor memory
+// and then waits, see wait_for_previous_kernel()).
 template <typename... Args>
 mxb_status launch_cluster(const char* what, void (*kernel)(Args...), unsigned clusters, unsigned size,
                           unsigned threads, size_t smem, cudaStream_t s,
@@ -46,12 +48,14 @@ mxb_status launch_cluster(const char* what, void (*kernel)(Args...), unsigned cl
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = size;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
   if (e != cudaSuccess) {
     (void)cudaGetLastError();

@@ -150,6 +150,17 @@ __device__ __forceinline__ void tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
+// ---- programmatic dependent launch
+// A kernel launched with the attribute may start while the kernel before it in the
+// stream is still running; it must wait before it touches global memory, reads and
+// writes alike.  Letting its own successor start is only a hint.
+__device__ __forceinline__ void wait_for_previous_kernel() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void allow_next_kernel() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // ---- thread-block clusters
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
