@@ -5,9 +5,11 @@ Layers, bottom-up:
   mxfp4_b200.capi       ctypes binding of that C ABI (no torch types)
   omo                   C++ torch extension with the reference's op names
   omo_python_api        the reference's Python wrappers (allocation, padding,
-                        splits) on top of `omo`
+                        splits) on top of `omo`; mxfp4_moe: the operators of
+                        a mixture-of-experts layer's experts
   mxfp4_b200.ep         MoE expert-parallel dispatch / combine with MXFP4
                         payloads over torch.distributed (NCCL)
+  mxfp4_b200.moe        the experts as an autograd layer
 """
 from __future__ import annotations
 
