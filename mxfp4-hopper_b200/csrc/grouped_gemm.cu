@@ -736,8 +736,8 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) grouped_narrow_kernel(
       const int rows = min(kT, g.off[tl.e + 1] - tl.m0);
       const int buf = i & 1;
       bool ok = mbar_wait_suspend(&acc_full[buf], (uint32_t)((i / 2) & 1));
-      // every owner has summed tile i - 1
-      if (i > 0) ok = mbar_wait_cluster(part_empty, (uint32_t)((i - 1) & 1)) && ok;
+      // every owner has summed tile i - 1 (alone, this CTA's barrier below says so)
+      if (i > 0 && ranks > 1) ok = mbar_wait_cluster(part_empty, (uint32_t)((i - 1) & 1)) && ok;
       tc_fence_after();
       if (!ok) atomicExch(failed, 1);
       __syncwarp();
@@ -749,22 +749,30 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) grouped_narrow_kernel(
           tmem_ld16(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)((buf * kBlocks + b) * kT + c),
                     acc);
           tmem_ld_wait();
+          if (ranks == 1) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            peer_store(to + (uint32_t)((b * kT + c + j) * cols * 4), __uint_as_float(acc[j]));
+            for (int j = 0; j < 16; ++j)
+              part[(b * kT + c + j) * 128 + n_acc] = __uint_as_float(acc[j]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              peer_store(to + (uint32_t)((b * kT + c + j) * cols * 4), __uint_as_float(acc[j]));
+          }
         }
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&acc_empty[buf]);
-      named_sync(1, 128);
-      if (et < (int)ranks) {
-        fence_cluster();
-        peer_arrive(peer_addr(smem_addr(part_full), (uint32_t)et));
+      if (ranks > 1) {
+        named_sync(1, 128);
+        if (et < (int)ranks) {
+          fence_cluster();
+          peer_arrive(peer_addr(smem_addr(part_full), (uint32_t)et));
+        }
+        __syncwarp();
+        ok = mbar_wait_cluster(part_full, (uint32_t)(i & 1));
+        if (!ok) atomicExch(failed, 1);
       }
-      __syncwarp();
-      ok = mbar_wait_cluster(part_full, (uint32_t)(i & 1));
-      if (!ok) atomicExch(failed, 1);
       // a wait that gave up ends the tiles of this CTA; its peers give up in turn
       if (named_sync_or(1, 128, !ok || *((volatile int*)failed))) break;
       {
@@ -815,7 +823,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) grouped_narrow_kernel(
       }
       // the partial sums have been read
       named_sync(1, 128);
-      if (et < (int)ranks) {
+      if (ranks > 1 && et < (int)ranks) {
         fence_cluster();
         peer_arrive(peer_addr(smem_addr(part_empty), (uint32_t)et));
       }
@@ -916,15 +924,16 @@ int64_t most_tiles(int64_t M, int64_t E, int rows, int64_t ntn) {
 Plan grouped_plan(const GroupedArgs& p, bool glu) {
   const int sms = sm_count();
   const int64_t ksteps = cdiv(p.K, kStepK);
-  const int64_t wide = most_tiles(p.M, p.E, 256, cdiv(p.width, glu ? 128 : 256));
-  Plan r{256, 1, wide};
-  if (p.M > 96 * (int64_t)p.E && wide >= sms / 2) return r;
-  r.rows = p.M <= 8 * (int64_t)p.E ? 16 : 64;
+  Plan r{p.M <= 8 * (int64_t)p.E ? 16 : 64, 1, 0};
   r.tiles = most_tiles(p.M, p.E, r.rows, cdiv(p.width, 128));
+  // Wide from about 96 rows an expert, unless the narrow tiles are one round at most
+  // (then they may also split K).  500 rows of 4096 x 4096: wide 19 us, narrow 27.
+  if (p.M > 96 * (int64_t)p.E && r.tiles > sms)
+    return Plan{256, 1, most_tiles(p.M, p.E, 256, cdiv(p.width, glu ? 128 : 256))};
   const int most = p.c_codes ? 4 : 8;  // a quantized block of 32 columns has one owner
   while (r.ranks < most && r.tiles * r.ranks * 2 <= sms && ksteps >= r.ranks * 4) r.ranks *= 2;
   // long tiles in a few rounds that read each weight for a few rows: half tiles fill
-  // the last round better
+  // the last round better (128 rows over 32 experts of 4096 x 7168: 82 -> 77 us)
   if (r.ranks == 1 && ksteps >= 16 && p.M <= 32 * (int64_t)p.E && r.tiles <= 8 * sms) r.ranks = 2;
   return r;
 }
