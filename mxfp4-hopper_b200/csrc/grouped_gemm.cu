@@ -129,13 +129,14 @@ __device__ __forceinline__ float load_bias(const GroupedArgs& p, int64_t i) {
 
 // ---------------------------------------------------------------- wide
 // A persistent pair of CTAs (cta_group::2) per two SMs; a tile has 256 rows, 128
-// in each CTA, and 256 weight rows, of which each CTA holds 128: columns n0 ..
-// n0 + 255 of the result, or (gated) the gate and the up rows of columns n0 ..
-// n0 + 127.  Each operand byte crosses L2 -> shared memory once per 256 x 256
-// tile instead of once per 128 x 256.
+// in each CTA, and kN weight rows, of which each CTA holds half: columns n0 ..
+// n0 + kN - 1 of the result, or (gated) the gate and the up rows of columns n0 ..
+// n0 + kN / 2 - 1.  kN is 256, where each operand byte crosses L2 -> shared memory
+// once per 256 x 256 tile instead of once per 128 x 256, or 128, where twice the
+// tiles fill the GPU better.
 //   warp 0       TMA of this CTA's half of A's and B's codes, completing on CTA
 //                0's barrier
-//   warp 1       (CTA 0) MMA issue: four M = 256, N = 256, K = 64 a step
+//   warp 1       (CTA 0) MMA issue: four M = 256, N = kN, K = 64 a step
 //   warp 2       scales of four K steps at a time: a TMA box of 32 bytes of each
 //                of A's rows, bulk copies of B's atoms (both halves)
 //   warps 4-7    scales: each warp gathers its lane quadrant's words of a step
@@ -168,7 +169,7 @@ static_assert(kWideStage % 1024 == 0, "swizzled boxes start on 1024 bytes");
 // scale warps must not spill: a spilled load is waited for where it is issued.
 constexpr int kWideCopyRegs = 64, kWideScaleRegs = 96, kWideEpilogueRegs = 176;
 
-template <int kAct>
+template <int kAct, int kN>
 __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
     const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
     const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ GroupedArgs p) {
@@ -191,7 +192,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
   g.tile = g.off + p.E + 1;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const int rank = (int)cluster_rank();
-  constexpr int kTileN = kGlu ? 128 : 256;
+  constexpr int kTileN = kGlu ? kN / 2 : kN;
+  constexpr uint32_t kBBox = kN / 2 * 128;  // this CTA's weight rows of a stage
+  // 128-row scale blocks a tile reads: two, but one for 128 columns of a plain result
+  constexpr bool kTwoBlocks = kGlu || kN == 256;
   const int ntn = (p.width + kTileN - 1) / kTileN;
   const int ksteps = (p.K + kStepK - 1) / kStepK;
   const int S = p.K / 32, S4 = (S + 3) / 4;
@@ -239,9 +243,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
     return r;
   };
 
-  // columns 128 .. 255 of a plain tile may all lie past the result: then CTA 1's
-  // weight rows are not loaded and its stale codes make columns that are not written
-  auto has_second = [&](const Tile& tl) { return kGlu || tl.n0 + 128 < p.width; };
+  // columns 128 .. 255 of a plain tile may all lie past the result: then their scales
+  // and CTA 1's weight rows are not loaded, and what is stale there makes columns that
+  // are not written
+  auto has_second = [&](const Tile& tl) { return kGlu || kN == 128 || tl.n0 + 128 < p.width; };
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideCopyRegs));
@@ -253,7 +258,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
       for (int i = 0; ok && i < my_tiles; ++i) {
         const Tile tl = tile_at(i);
         const int row = kGlu ? (2 * tl.e + rank) * p.width + tl.n0
-                             : tl.e * p.width + tl.n0 + 128 * rank;
+                             : tl.e * p.width + tl.n0 + kN / 2 * rank;
         const bool second = has_second(tl);
         for (int ks = 0; ks < ksteps; ++ks, ++gs) {
           const int s = gs % kWideStages;
@@ -263,7 +268,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
             break;
           }
           uint8_t* st = smem + s * kWideStage;
-          if (rank == 0) mbar_arrive_expect_tx(&full[s], (second ? 4 : 3) * kBoxBytes);
+          if (rank == 0)
+            mbar_arrive_expect_tx(&full[s], 2 * kBoxBytes + (second ? 2 : 1) * kBBox);
           const int kx = ks * (kStepK / 2);
           tma_load_2d_pair(st, &map_a, kx, tl.m0, full0 + 8 * s);
           if (rank == 0 || second) tma_load_2d_pair(st + kBoxBytes, &map_b, kx, row, full0 + 8 * s);
@@ -292,10 +298,11 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
           }
           uint8_t* sb = scales + s * kSbStage;
           const uint32_t atoms = (uint32_t)min(8, S4 - k4) * 512;
-          mbar_arrive_expect_tx(&sb_full[s], (p.a_scales_tma ? kSbA : 0) + (second ? 2 : 1) * atoms);
+          const bool two = kTwoBlocks && second;
+          mbar_arrive_expect_tx(&sb_full[s], (p.a_scales_tma ? kSbA : 0) + (two ? 2 : 1) * atoms);
           if (p.a_scales_tma) tma_load_2d(sb, &map_sa, 4 * k4, tl.m0, &sb_full[s]);
           bulk_load_1d(sb + kSbA, src0 + k4 * 512, atoms, &sb_full[s]);
-          if (second) bulk_load_1d(sb + kSbA + kSbB, src1 + k4 * 512, atoms, &sb_full[s]);
+          if (two) bulk_load_1d(sb + kSbA + kSbB, src1 + k4 * 512, atoms, &sb_full[s]);
         }
       }
       for (int q = gq > kSbStages ? gq - kSbStages : 0; q < gq; ++q)
@@ -331,8 +338,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
             if (64 * j >= left) break;
             const uint32_t sf_id = (uint32_t)(j & 1) * 2u;
             tc_mma_pair(tmem, da + (uint64_t)(2 * j), db + (uint64_t)(2 * j),
-                        mxf4_idesc(256, 256, sf_id), (sfc + 4 * (j >> 1)) | (sf_id << 30),
-                        (sfc + 8 + 8 * (j >> 1)) | (sf_id << 30), (ks > 0 || j > 0) ? 1u : 0u, one);
+                        mxf4_idesc(256, kN, sf_id), (sfc + 4 * (j >> 1)) | (sf_id << 30),
+                        (sfc + 8 + kN / 32 * (j >> 1)) | (sf_id << 30),
+                        (ks > 0 || j > 0) ? 1u : 0u, one);
           }
           tc_commit_pair(&empty[s], one);
         }
@@ -351,7 +359,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
     int gs = 0, gq = 0;
     bool ok = true;
     for (int i = 0; ok && i < my_tiles; ++i) {
-      const int64_t row0 = p.a_scales_tma ? 0 : (int64_t)tile_at(i).m0 + 32 * q;
+      const Tile tl = tile_at(i);
+      const int64_t row0 = (int64_t)tl.m0 + 32 * q;
       for (int ks0 = 0; ok && ks0 < ksteps; ks0 += 4, ++gq) {
         const int sq = gq % kSbStages;
         uint8_t* sb = scales + sq * kSbStage;
@@ -378,13 +387,30 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
                                    h ? ra[2].z : ra[2].x, h ? ra[3].z : ra[3].x,
                                    h ? ra[0].w : ra[0].y, h ? ra[1].w : ra[1].y,
                                    h ? ra[2].w : ra[2].y, h ? ra[3].w : ra[3].y};
-            // the columns of one K atom of B's two halves are neighbours
-            uint32_t b[16];
+            // a column of B's scales is 32 of its kN rows; the columns of one K atom are
+            // neighbours: 4 + 4 of two blocks, 4 of one, or (gated, kN = 128) the two
+            // halves' 2 + 2 columns from where n0 lies in their blocks
+            uint32_t b[kN / 16];
+            const uint8_t* sbb = sb + kSbA + 2 * (j + h) * 512 + lane * 16;
+            if constexpr (kN == 256) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint4 w = *reinterpret_cast<const uint4*>(
-                  sb + kSbA + (k & 1) * kSbB + (2 * (j + h) + (k >> 1)) * 512 + lane * 16);
-              b[4 * k] = w.x; b[4 * k + 1] = w.y; b[4 * k + 2] = w.z; b[4 * k + 3] = w.w;
+              for (int k = 0; k < 4; ++k) {
+                const uint4 w = *reinterpret_cast<const uint4*>(sbb + (k & 1) * kSbB + (k >> 1) * 512);
+                b[4 * k] = w.x; b[4 * k + 1] = w.y; b[4 * k + 2] = w.z; b[4 * k + 3] = w.w;
+              }
+            } else if constexpr (kGlu) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint2 w = *reinterpret_cast<const uint2*>(
+                    sbb + (k & 1) * kSbB + (k >> 1) * 512 + (tl.n0 & 64) / 8);
+                b[2 * k] = w.x; b[2 * k + 1] = w.y;
+              }
+            } else {
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const uint4 w = *reinterpret_cast<const uint4*>(sbb + k * 512);
+                b[4 * k] = w.x; b[4 * k + 1] = w.y; b[4 * k + 2] = w.z; b[4 * k + 3] = w.w;
+              }
             }
             const int s = gs % kWideStages;
             up = up && (gs < kWideStages ||
@@ -392,7 +418,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
             tc_fence_after();
             __syncwarp();
             tmem_st8(col0 + (uint32_t)(s * 24), a);
-            tmem_st16(col0 + (uint32_t)(s * 24 + 8), b);
+            if constexpr (kN == 256) tmem_st16(col0 + (uint32_t)(s * 24 + 8), b);
+            else tmem_st8(col0 + (uint32_t)(s * 24 + 8), b);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -415,6 +442,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
     const int r = quad * 32 + lane, ht = t & 127;
     float* bias_h = bias_s + half * 128;
     constexpr int kHalfN = kTileN / 2;  // result columns of this group
+    constexpr int kAcc = kN / 2;        // its accumulator columns: of z, or gate then up
+    constexpr int kUp = kAcc / 2;       // where up starts among them
     const uint32_t acc_empty0 = peer_addr(smem_addr(acc_empty), 0);
     const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
     const bool c32 = sectors(p.c, p.c_ld), pre32 = sectors(p.pre, p.pre_ld) && p.width % 16 == 0;
@@ -425,10 +454,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
       const int nh = tl.n0 + half * kHalfN;                // first result column of this group
       const bool mine = r < rows;
       float bias = 0.0f;
-      if (p.bias) {
-        // this group's 128 accumulator columns: 128 of z, or 64 gate and 64 up
-        const int col = kGlu ? nh + (ht & 63) : nh + ht;
-        const int64_t at = kGlu ? (int64_t)tl.e * 2 * p.width + (ht < 64 ? 0 : p.width) + col
+      if (p.bias && ht < kAcc) {
+        const int col = nh + (kGlu ? ht % kUp : ht);
+        const int64_t at = kGlu ? (int64_t)tl.e * 2 * p.width + (ht < kUp ? 0 : p.width) + col
                                 : (int64_t)tl.e * p.width + col;
         if (col < p.width) bias = load_bias(p, at);
       }
@@ -446,13 +474,13 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
       tc_fence_after();
       const bool live = ok && !*((volatile int*)failed);
       if (named_sync_or(1 + half, 128, !live)) break;  // the four warps leave together
-      uint32_t acc[128];
+      uint32_t acc[kAcc];
       __syncwarp();
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        tmem_ld32(lane_base + (uint32_t)(kGlu ? (k >> 1) * 128 + half * 64 + (k & 1) * 32
-                                              : half * 128 + k * 32),
-                  acc + 32 * k);
+      for (int k = 0; k < kAcc; k += 32)
+        tmem_ld32(lane_base + (uint32_t)(kGlu ? k / kUp * (kN / 2) + half * kUp + k % kUp
+                                              : half * kAcc + k),
+                  acc + k);
       tmem_ld_wait();
       tc_fence_before();
       __syncwarp();
@@ -474,15 +502,15 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
         };
         add_bias(acc, bias_h + 32 * ch, v);
         if constexpr (kGlu) {
-          add_bias(acc + 64, bias_h + 64 + 32 * ch, u);
+          add_bias(acc + kUp, bias_h + kUp + 32 * ch, u);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
+          for (int j = 0; j + 32 < kUp; ++j) {
             acc[j] = acc[32 + j];
-            acc[64 + j] = acc[96 + j];
+            acc[kUp + j] = acc[kUp + 32 + j];
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < 96; ++j) acc[j] = acc[32 + j];
+          for (int j = 0; j + 32 < kAcc; ++j) acc[j] = acc[32 + j];
         }
         uint32_t w[16];
         if (p.pre) {
@@ -914,6 +942,7 @@ __global__ void __launch_bounds__(256) swizzle_grouped_kernel(const uint8_t* __r
 struct Plan {
   int rows, ranks;
   int64_t tiles;  // upper bound over all splits
+  int n = 0;      // wide: weight rows of a tile
 };
 
 int64_t most_tiles(int64_t M, int64_t E, int rows, int64_t ntn) {
@@ -921,32 +950,70 @@ int64_t most_tiles(int64_t M, int64_t E, int rows, int64_t ntn) {
   return (groups + (M - groups) / rows) * ntn;
 }
 
+// Few rows an expert (the weights' bytes are the time): narrow.  Else the least of three
+// estimates in tenths of a microsecond, each a start with the last tile's epilogue, so
+// much a K step, and a further round of tiles at the longer of its steps and an
+// epilogue; at least the weights' bytes at the rate each reaches.  The coefficients were
+// read off products of 40 to 8192 rows, e.g. (us, narrow / 128 / 256 weight rows a
+// tile): 200 x 1024 x 256 7.9 / 6.3 / 8.5; 300 x 3600 x 4096 13.3 / 9.6 / 13.1;
+// 130 x 512 x 7168, where narrow splits K eight ways, 8.8 / 11.2 / 16.0;
+// 1500 x 2048 x 2048 19.4 / 10.5 / 12.0; 2000 x 4096 x 4096 43.9 / 23.9 / 21.5;
+// 1500 rows over 32 experts of 4096 x 7168 96 / 132 / 103.
 Plan grouped_plan(const GroupedArgs& p, bool glu) {
-  const int sms = sm_count();
-  const int64_t ksteps = cdiv(p.K, kStepK);
+  const int sms = sm_count(), pairs = std::max(1, sms / 2);
+  const int64_t ksteps = cdiv(p.K, kStepK), cols = (int64_t)p.width * (glu ? 2 : 1);
+  const int64_t groups = std::min<int64_t>(p.E, p.M);  // experts with rows, at most
+  // row blocks of an even split
+  auto blocks = [&](int rows) {
+    return p.E == 1 ? cdiv(p.M, rows) : std::max(groups, p.M / rows + cdiv(groups, 2));
+  };
   Plan r{p.M <= 8 * (int64_t)p.E ? 16 : 64, 1, 0};
   r.tiles = most_tiles(p.M, p.E, r.rows, cdiv(p.width, 128));
-  // Wide from about 96 rows an expert, unless the narrow tiles are one round at most
-  // (then they may also split K).  500 rows of 4096 x 4096: wide 19 us, narrow 27.
-  if (p.M > 96 * (int64_t)p.E && r.tiles > sms)
-    return Plan{256, 1, most_tiles(p.M, p.E, 256, cdiv(p.width, glu ? 128 : 256))};
   const int most = p.c_codes ? 4 : 8;  // a quantized block of 32 columns has one owner
   while (r.ranks < most && r.tiles * r.ranks * 2 <= sms && ksteps >= r.ranks * 4) r.ranks *= 2;
-  // long tiles in a few rounds that read each weight for a few rows: half tiles fill
-  // the last round better (128 rows over 32 experts of 4096 x 7168: 82 -> 77 us)
-  if (r.ranks == 1 && ksteps >= 16 && p.M <= 32 * (int64_t)p.E && r.tiles <= 8 * sms) r.ranks = 2;
-  return r;
+  if (p.M <= 32 * (int64_t)p.E) {
+    // long tiles in a few rounds: half tiles fill the last round better (128 rows over
+    // 32 experts of 4096 x 7168: 82 -> 77 us)
+    if (r.ranks == 1 && ksteps >= 16 && r.tiles <= 8 * sms) r.ranks = 2;
+    return r;
+  }
+  // start, rounds, a step's cost in hundredths, a round's least
+  auto estimate = [&](int64_t start, int64_t rounds, int64_t steps, int64_t step, int64_t least) {
+    const int64_t tile = steps * step / 10;
+    return start + tile + (rounds - 1) * std::max(least, tile + 5);
+  };
+  const int64_t weights = groups * cols * p.K * 17 / 32;
+  const int64_t narrow =
+      std::max(estimate(r.ranks > 1 ? 85 : 70, cdiv(blocks(64) * cdiv(p.width, 128) * r.ranks, sms),
+                        cdiv(ksteps, r.ranks), glu ? 56 : 35, 35),
+               weights / 580000);
+  // rows of scales that TMA cannot take are gathered once per tile
+  const int64_t wide128 = std::max(estimate(60, cdiv(blocks(256) * cdiv(cols, 128), pairs), ksteps,
+                                            p.a_scales_tma ? 21 : 50, 22),
+                                   weights / 490000);
+  const int64_t wide256 = std::max(estimate(85, cdiv(blocks(256) * cdiv(cols, 256), pairs), ksteps,
+                                            p.a_scales_tma ? 31 : 50, 47),
+                                   weights / 490000);
+  if (narrow <= std::min(wide128, wide256)) return r;
+  const int n = wide128 < wide256 ? 128 : 256;
+  return Plan{256, 1, most_tiles(p.M, p.E, 256, cdiv(cols, n)), n};
 }
 
+template <int kAct, int kN>
+mxb_status launch_wide_n(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& ts,
+                       const GroupedArgs& p, const Plan& plan, cudaStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  MXB_REQUIRE(grant_smem((const void*)grouped_wide_kernel<kAct, kN>, kWideSmem, done), MXB_ERR_CUDA,
+              "grouped_gemm_mxfp4: cannot reserve shared memory");
+  return launch_cluster("grouped_gemm_mxfp4", grouped_wide_kernel<kAct, kN>,
+                        (unsigned)std::min<int64_t>(plan.tiles, std::max(1, sm_count() / 2)), 2,
+                        kWideThreads, kWideSmem, s, ta, tb, ts, p);
+}
 template <int kAct>
 mxb_status launch_wide(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& ts,
                        const GroupedArgs& p, const Plan& plan, cudaStream_t s) {
-  static std::atomic<uint64_t> done{0};
-  MXB_REQUIRE(grant_smem((const void*)grouped_wide_kernel<kAct>, kWideSmem, done), MXB_ERR_CUDA,
-              "grouped_gemm_mxfp4: cannot reserve shared memory");
-  return launch_cluster("grouped_gemm_mxfp4", grouped_wide_kernel<kAct>,
-                        (unsigned)std::min<int64_t>(plan.tiles, std::max(1, sm_count() / 2)), 2,
-                        kWideThreads, kWideSmem, s, ta, tb, ts, p);
+  return plan.n == 128 ? launch_wide_n<kAct, 128>(ta, tb, ts, p, plan, s)
+                       : launch_wide_n<kAct, 256>(ta, tb, ts, p, plan, s);
 }
 
 template <bool kGlu, int kT>
@@ -1047,7 +1114,7 @@ extern "C" mxb_status mxb_grouped_gemm_mxfp4(const void* a_codes, int64_t a_code
   p.c_ld = ep->c_ld;
   p.c_codes = (uint8_t*)ep->c_codes;
   p.c_scales = (uint8_t*)ep->c_scales;
-  p.a_scales_tma = 0;
+  p.a_scales_tma = aligned(a_scales, 16) && a_scales_pitch % 16 == 0;
   const Plan plan = grouped_plan(p, glu);
   MXB_REQUIRE(plan.tiles <= INT32_MAX, MXB_ERR_INVALID_ARGUMENT, "%s: too many tiles", what);
 
@@ -1056,7 +1123,7 @@ extern "C" mxb_status mxb_grouped_gemm_mxfp4(const void* a_codes, int64_t a_code
   if (!make_tensor_map_2d(&ta, a_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, M, K / 2, a_codes_pitch,
                           128, (uint32_t)std::min(plan.rows, 128), CU_TENSOR_MAP_SWIZZLE_128B) ||
       !make_tensor_map_2d(&tb, b_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (int64_t)E * N, K / 2,
-                          K / 2, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B))
+                          K / 2, 128, plan.n == 128 ? 64 : 128, CU_TENSOR_MAP_SWIZZLE_128B))
     return MXB_ERR_CUDA;
   if (plan.rows == 16)
     return glu ? launch_narrow<true, 16>(ta, tb, p, plan, s)
@@ -1065,7 +1132,6 @@ extern "C" mxb_status mxb_grouped_gemm_mxfp4(const void* a_codes, int64_t a_code
     return glu ? launch_narrow<true, 64>(ta, tb, p, plan, s)
                : launch_narrow<false, 64>(ta, tb, p, plan, s);
   CUtensorMap ts = ta;
-  p.a_scales_tma = aligned(a_scales, 16) && a_scales_pitch % 16 == 0;
   if (p.a_scales_tma && !make_tensor_map_2d(&ts, a_scales, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, M,
                                             K / 32, a_scales_pitch, 32, 128))
     return MXB_ERR_CUDA;

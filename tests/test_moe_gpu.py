@@ -46,7 +46,8 @@ def weights(E, N, K, seed, gated):
     return bc, bs, moe.omo_swizzle_scales_grouped(bs, gated)
 
 
-# every kernel: rows per expert <= 24 (16-row tiles), more (64-row tiles), many (wide)
+# every kernel: few rows an expert (16- and 64-row tiles, alone and splitting K), many (wide
+# tiles of 128 and, with long K or scale rows that TMA cannot take, 256 weight rows)
 GROUPED = [
     # E, M, N, K
     (1, 1, 64, 32),
@@ -61,6 +62,12 @@ GROUPED = [
     (2, 1000, 4400, 96),
     (1, 200, 19200, 256),
     (5, 3001, 1424, 544),
+    (1, 30, 1032, 2048),
+    (1, 60, 336, 7200),
+    (3, 300, 72, 9216),
+    (3, 2600, 2600, 4096),
+    (4, 2000, 4400, 2080),
+    (2, 1500, 4400, 3712),
 ]
 
 
@@ -90,7 +97,8 @@ def test_grouped(cuda, E, M, N, K, name):
 
 
 @pytest.mark.parametrize("name", ["none", "gelu", "swiglu"])
-@pytest.mark.parametrize("E,M,W,K", [(4, 30, 96, 1024), (2, 90, 160, 288), (3, 1500, 2368, 128)])
+@pytest.mark.parametrize("E,M,W,K", [(4, 30, 96, 1024), (2, 90, 160, 288), (3, 1500, 2368, 128),
+                                     (3, 2600, 1312, 4096)])
 def test_quantized_result_is_the_quantizer_on_c(cuda, E, M, W, K, name):
     N = 2 * W if name == "swiglu" else W
     splits = splits_of(E, M, W + M)
@@ -135,8 +143,9 @@ def test_dense_equals_the_plain_gemm(cuda):
     (3000, [700, 1400, 0, 300]),
     (3000, [2000, 2000, 2 ** 31 - 1, 2 ** 31 - 1]),
 ])
-def test_rows_outside_the_splits_are_left_alone(cuda, M, splits):
-    N, K = 4800 if M == 3000 else 160, 96
+@pytest.mark.parametrize("K", [96, 2080])
+def test_rows_outside_the_splits_are_left_alone(cuda, M, splits, K):
+    N = 4800 if M == 3000 else 160
     ac, asc = R.mxfp4(M, K, 1)
     bc, bs, bt = weights(4, N, K, 2, False)
     mark = torch.full((M, N), 3.0, dtype=BF, device=cuda)
@@ -151,8 +160,9 @@ def test_rows_outside_the_splits_are_left_alone(cuda, M, splits):
         R.check(x, y, torch.where(torch.isnan(by), 1e-30, by))
 
 
-@pytest.mark.parametrize("K", [256, 160])
-@pytest.mark.parametrize("E,M,N", [(3, 20, 96), (2, 150, 96), (2, 1200, 4800)])
+@pytest.mark.parametrize("E,M,N,K", [(3, 20, 96, 256), (3, 20, 96, 160), (2, 150, 96, 256), (2, 150, 96, 160),
+                                     (2, 1200, 4800, 256), (2, 1200, 4800, 160), (4, 2000, 4400, 2080),
+                                     (3, 2600, 2600, 4096)])
 def test_strided_rows_and_pitches(cuda, E, M, N, K):
     """Wire rows (codes and scales side by side) as A, and padded c, pre and residual."""
     splits = splits_of(E, M, 7)
@@ -172,7 +182,7 @@ def test_strided_rows_and_pitches(cuda, E, M, N, K):
     assert (big[:2, :, :8] == 7).all() and (big[:2, :, 8 + N:] == 7).all()
 
 
-@pytest.mark.parametrize("K", [512, 384, 288])
+@pytest.mark.parametrize("K", [512, 384, 288, 4096])
 @pytest.mark.parametrize("E,M,N", [(3, 20, 96), (2, 150, 96), (2, 1200, 4800)])
 def test_scale_rows_at_any_address(cuda, E, M, N, K):
     """A's scale rows at an odd base and pitch give the same bytes as aligned ones."""
@@ -187,10 +197,10 @@ def test_scale_rows_at_any_address(cuda, E, M, N, K):
         assert torch.equal(got.view(torch.int16), want.view(torch.int16))
 
 
-@pytest.mark.parametrize("E,M,N", [(3, 20, 96), (3, 150, 96), (3, 1300, 4800)])
-def test_nan_scales_stay_in_their_row(cuda, E, M, N):
+@pytest.mark.parametrize("E,M,N,K", [(3, 20, 96, 320), (3, 150, 96, 320), (3, 1300, 4800, 320),
+                                     (3, 2600, 2600, 4096), (4, 2000, 4400, 2080)])
+def test_nan_scales_stay_in_their_row(cuda, E, M, N, K):
     """A row or weight row whose E8M0 byte is NaN (255) makes its own results NaN only."""
-    K = 320
     splits = splits_of(E, M, 3)
     ac, asc = R.mxfp4(M, K, 1)
     bc, bs, _ = weights(E, N, K, 2, False)
