@@ -200,7 +200,6 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
   const int ksteps = (p.K + kStepK - 1) / kStepK;
   const int S = p.K / 32, S4 = (S + 3) / 4;
 
-  allow_next_kernel();
   if (warp == 0) {
     wait_for_previous_kernel();
     build_groups(g, p.m_splits, p.E, p.M, [&](int rows) { return (rows + 255) / 256 * ntn; });
@@ -224,6 +223,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
   __syncthreads();
   tc_fence_after();
   cluster_sync();
+  allow_next_kernel();  // every CTA of this one has its tensor memory
   wait_for_previous_kernel();
   const uint32_t tmem = *tmem_slot;
   const int tiles = g.tile[p.E];
@@ -581,7 +581,11 @@ struct Narrow {
   // Four stages: 128 rows over 32 experts of 4096 x 7168 take 77 us with 3 or 4, 81
   // with the 5 that fit, and one row of 7168 x 2048 8.5 us with 4, 8.8 with 9.
   static constexpr int kStages = kMost > 4 ? 4 : kMost;
-  static constexpr size_t kSmem = kFixed + kStages * kStage;
+  // More than half of an SM's shared memory: two CTAs that own tensor memory never share
+  // an SM.  (The second would wait in its allocation, and two clusters that each got one
+  // of two SMs' tensor memory would wait for each other.)
+  static constexpr size_t kNeeded = kFixed + kStages * kStage;
+  static constexpr size_t kSmem = kNeeded < 116 * 1024 ? 116 * 1024 : kNeeded;
   static constexpr uint32_t kScaleCols = kBlocks * 8 + 8;
   static_assert(kStages >= 3 && 2 * kBlocks * kT <= 256 && 256 + kStages * kScaleCols <= kTmemCols,
                 "the ring and tensor memory fit");
@@ -616,7 +620,6 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) grouped_narrow_kernel(
   const int k_end = (int)((int64_t)ksteps * (rank + 1) / ranks);
   const int S = p.K / 32, S4 = (S + 3) / 4;
 
-  allow_next_kernel();
   if (warp == 0) {
     wait_for_previous_kernel();
     build_groups(g, p.m_splits, p.E, p.M, [&](int rows) { return (rows + kT - 1) / kT * ntn; });
@@ -641,6 +644,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) grouped_narrow_kernel(
   __syncthreads();
   tc_fence_after();
   cluster_sync();  // every CTA's barriers are ready for its peers
+  allow_next_kernel();  // every CTA of this one has its tensor memory
   wait_for_previous_kernel();
   const uint32_t tmem = *tmem_slot;
   const int tiles = g.tile[p.E];

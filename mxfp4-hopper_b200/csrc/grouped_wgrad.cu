@@ -109,7 +109,6 @@ __global__ void __launch_bounds__(kWgThreads, 1) grouped_wgrad_kernel(
   const int per_expert = nty * ntx;
   const int rank = (int)cluster_rank();
 
-  allow_next_kernel();
   if (warp == 0) {
     wait_for_previous_kernel();
     build_groups(g, p.m_splits, p.E, p.M, [&](int) { return 0; });
@@ -132,6 +131,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) grouped_wgrad_kernel(
   __syncthreads();
   tc_fence_after();
   cluster_sync();
+  allow_next_kernel();  // every CTA of this one has its tensor memory
   wait_for_previous_kernel();
   const uint32_t tmem = *tmem_slot;
   const int tiles = p.E * per_expert;

@@ -153,7 +153,8 @@ __device__ __forceinline__ void tmem_st_wait() {
 // ---- programmatic dependent launch
 // A kernel launched with the attribute may start while the kernel before it in the
 // stream is still running; it must wait before it touches global memory, reads and
-// writes alike.  Letting its own successor start is only a hint.
+// writes alike.  Letting its own successor start is a hint, given once this CTA has its
+// tensor memory: a successor that allocated first could hold up a cluster of this one.
 __device__ __forceinline__ void wait_for_previous_kernel() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }

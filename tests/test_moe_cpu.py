@@ -78,7 +78,7 @@ def unpg(d=A, y=A, R=16, H=64, m=A, mp=2, k=2, w=A, T=8, dy=A, q=None, s=None, d
     (grad(dz=None, db=None), 1, "no output"),
     (grad(pre=None), 1, "null"),
     (grad(m=None), 1, "null"),
-    (grad(M=33), 1, "workspace"),
+    (grad(M=513), 1, "workspace"),
     (grad(dy=A + 8), 2, "aligned"),
     (unp(H=60), 1, "H"),
     (unp(k=0), 1, "topk"),
@@ -110,8 +110,8 @@ def test_empty_calls_do_nothing(call):
 
 def test_workspace_size():
     f = capi.load().mxb_bias_act_grad_workspace
-    assert f(32, 8, 4096) == 0           # one block of rows per expert: no partial sums
-    assert f(33, 8, 4096) == 9 * 4096 * 4
+    assert f(512, 8, 4096) == 0          # a cluster has an expert's rows: no partial sums
+    assert f(513, 8, 4096) == (16 + 8) * 4096 * 4
     assert f(16384, 8, 4096) == (128 + 8) * 4096 * 4
 
 
