@@ -55,20 +55,13 @@ struct WgradArgs {
 };
 
 // 32 codes (16 bytes) and their E8M0 byte -> 32 BF16 values in element order.
-// The eight magnitudes times 2^(e - 127) are made first (exact: a BF16 multiply by
-// the power of two, whose pattern is e << 7; past BF16's range they are infinite;
-// e = 0 halves first and scales by 2^-126, as 2^-127 has no normal pattern; e = 255
-// is the E8M0 NaN) and split into tables of low and high bytes, which prmt looks up
-// for four codes at a time.
+// The eight magnitudes times 2^(e - 127) are made first and split into tables of low
+// and high bytes, which prmt looks up for four codes at a time.  The factor's BF16
+// pattern is e << 7, for e = 0 the subnormal 0x40 (BF16 multiplies take subnormals): the
+// products are exact, past BF16's range infinite.  e = 255 is the E8M0 NaN.
 __device__ __forceinline__ void expand32(uint4 codes, uint32_t e, uint32_t (&out)[16]) {
+  const uint32_t f = (e == 255u ? 0x7FFFu : max(e << 7, 0x40u)) * 0x10001u;
   uint32_t m[4] = {0x3F000000u, 0x3FC03F80u, 0x40404000u, 0x40C04080u};  // 0 .5 | 1 1.5 | 2 3 | 4 6
-  uint32_t f = e == 255u ? 0x7FFFu : e << 7;
-  if (e == 0u) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) m[i] = mul_bf16x2(m[i], 0x3F003F00u);
-    f = 1u << 7;
-  }
-  f |= f << 16;
 #pragma unroll
   for (int i = 0; i < 4; ++i) m[i] = mul_bf16x2(m[i], f);
   const uint32_t lo0 = prmt(m[0], m[1], 0x6420u), lo1 = prmt(m[2], m[3], 0x6420u);
@@ -285,71 +278,96 @@ __global__ void __launch_bounds__(kWgThreads, 1) grouped_wgrad_kernel(
     const int first = (warp - 6) >> 1, b = lane >> 3;
     const int r0 = ((warp - 6) & 1) * 32 + (lane & 7);
     const uint32_t full0 = peer_addr(smem_addr(full), 0);
-    struct At {
-      int i, st;  // tile, step in it
-      Tile tl;
-    };
+    const int64_t c8 = 8 * p.x_pitch, s8 = 8 * p.s_pitch;
+    int i = -1, left = 0;  // tile; its rows from this pair's step on
+    const uint8_t *cp = nullptr, *sp = nullptr;  // this lane's codes and scale in row r0 of the step
+    bool in_k = false;
     // moves n steps on; false when there are no more
-    auto move = [&](At& at, int n) {
-      at.st += n;
-      while (at.i < my_tiles && at.st >= at.tl.steps) {
-        at.st -= at.tl.steps;
-        if (++at.i < my_tiles) at.tl = tile_at(at.i);
+    auto move = [&](int n) {
+      left -= n * kWgRows;
+      if (left > 0) {
+        cp += n * 8 * c8;
+        sp += n * 8 * s8;
+        return true;
       }
-      return at.i < my_tiles;
+      // steps past this tile's last one are the next tiles' first ones
+      int over = -left / kWgRows;
+      Tile tl;
+      for (;;) {
+        if (++i >= my_tiles) return false;
+        tl = tile_at(i);
+        if (over < tl.steps) break;
+        over -= tl.steps;
+      }
+      left = tl.rows - over * kWgRows;
+      const int64_t row = (int64_t)tl.row0 + over * kWgRows + r0;
+      const int k = tl.x0 + rank * (kTileX / 2) + 32 * b;
+      in_k = k < p.K;
+      cp = p.x_codes + row * p.x_pitch + k / 2;
+      sp = p.x_scales + row * p.s_pitch + k / 32;
+      return true;
     };
     uint4 codes[4];
     uint32_t scale[4];
-    auto load = [&](const At& at) {
+    auto load = [&] {
+      if (left >= kWgRows && in_k) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        codes[j] = make_uint4(0u, 0u, 0u, 0u);
-        scale[j] = 127u;
-        const int in = at.st * kWgRows + r0 + 8 * j, k = at.tl.x0 + rank * (kTileX / 2) + 32 * b;
-        if (in < at.tl.rows && k < p.K) {
-          const int64_t row = (int64_t)at.tl.row0 + in;
-          codes[j] = __ldg(reinterpret_cast<const uint4*>(p.x_codes + row * p.x_pitch + k / 2));
-          scale[j] = __ldg(p.x_scales + row * p.s_pitch + k / 32);
+        for (int j = 0; j < 4; ++j) {
+          codes[j] = __ldg(reinterpret_cast<const uint4*>(cp + j * c8));
+          scale[j] = __ldg(sp + j * s8);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          codes[j] = make_uint4(0u, 0u, 0u, 0u);
+          scale[j] = 127u;
+          if (r0 + 8 * j < left && in_k) {
+            codes[j] = __ldg(reinterpret_cast<const uint4*>(cp + j * c8));
+            scale[j] = __ldg(sp + j * s8);
+          }
         }
       }
     };
-    At at{0, 0, {}};
-    if (my_tiles > 0) at.tl = tile_at(0);
-    bool more = move(at, first);
-    if (more) load(at);
+    // where this lane's 16-byte chunks go: its rows are the same modulo 8
+    uint32_t chunk[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      chunk[q] = (uint32_t)((b >> 1) * kWgBox + r0 * 128 + ((((b & 1) * 4 + q) ^ (r0 & 7)) << 4));
+    bool more = move(first);
+    if (more) load();
     for (int gs = first; more; gs += 4) {
       const int s = gs % kWgStages;
       uint8_t* stage = smem + s * kWgStage;
-      const int here = at.tl.rows - at.st * kWgRows;  // rows of the expert in this step
-      bool ok = gs < kWgStages || mbar_wait_suspend(&empty[s], (uint32_t)((gs / kWgStages - 1) & 1));
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t v[16];
-        expand32(codes[j], scale[j], v);
-        const int r = r0 + 8 * j;
-        uint8_t* box = stage + (b >> 1) * kWgBox + r * 128;
-        if (ok) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<uint4*>(box + ((((b & 1) * 4 + q) ^ (r & 7)) << 4)) =
-                make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-        }
-      }
-      more = move(at, 4);
-      if (more) load(at);
-      ok = ok && mbar_wait_suspend(&dy_full[s], (uint32_t)((gs / kWgStages) & 1));
-      if (!ok) {
+      const int here = left;  // rows of the expert from this step on
+      if (gs >= kWgStages && !mbar_wait_suspend(&empty[s], (uint32_t)((gs / kWgStages - 1) & 1))) {
         atomicExch(failed, 1);
         break;
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int r = r0 + 8 * j;
-        if (r >= here) {  // past the expert's last row: its four lanes clear dy's four half rows
-          uint8_t* dyr = stage + kWgX + (b >> 1) * kWgBox + r * 128 + (b & 1) * 64;
+        uint32_t v[16];
+        expand32(codes[j], scale[j], v);
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<uint4*>(dyr + 16 * q) = make_uint4(0u, 0u, 0u, 0u);
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<uint4*>(stage + chunk[q] + j * 1024) =
+              make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+      }
+      more = move(4);
+      if (more) load();
+      if (!mbar_wait_suspend(&dy_full[s], (uint32_t)((gs / kWgStages) & 1))) {
+        atomicExch(failed, 1);
+        break;
+      }
+      if (here < kWgRows) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = r0 + 8 * j;
+          if (r >= here) {  // past the expert's last row: its four lanes clear dy's four half rows
+            uint8_t* dyr = stage + kWgX + (b >> 1) * kWgBox + r * 128 + (b & 1) * 64;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<uint4*>(dyr + 16 * q) = make_uint4(0u, 0u, 0u, 0u);
+          }
         }
       }
       fence_proxy_async_smem();
