@@ -46,7 +46,7 @@ constexpr float kSqrt2OverPi = 0.7978845608028654f;
 constexpr float kGeluCubic = 0.044715f;
 constexpr float kInvSqrt2Pi = 0.3989422804014327f;
 
-// P of normal_tail(), lowest coefficient first.
+// P of q(z), lowest coefficient first.
 __host__ __device__ constexpr float tail_coeff(int c) {
   return c == 0   ? 0.11962930113077164f
          : c == 1 ? 0.12075395882129669f
@@ -58,28 +58,12 @@ __host__ __device__ constexpr float tail_coeff(int c) {
                   : 0.03567477688193321f;
 }
 
-// erfc(|z| / sqrt 2) / 2, the normal distribution's upper tail; gauss = exp(-z^2 / 2).
-__device__ __forceinline__ float normal_tail(float z, float& gauss) {
-  const float t = rcp_approx(fmaf(0.3f, fabsf(z), 1.0f));
-  float p = tail_coeff(7);
-#pragma unroll
-  for (int c = 6; c >= 0; --c) p = fmaf(p, t, tail_coeff(c));
-  gauss = ex2_approx(z * z * (-0.5f * kLog2e));
-  return p * t * gauss;
-}
-
+// One value of the activations that need no more than a few instructions.
 template <int kAct>
 __device__ __forceinline__ float act_value(float z) {
   if constexpr (kAct == MXB_ACT_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
   if constexpr (kAct == MXB_ACT_RELU2) return z > 0.0f ? z * z : (z != z ? z : 0.0f);
   if constexpr (kAct == MXB_ACT_SILU) return z * logistic(z);
-  if constexpr (kAct == MXB_ACT_GELU) {
-    float gauss;
-    const float q = normal_tail(z, gauss);
-    return z * (z > 0.0f ? 1.0f - q : q);
-  }
-  if constexpr (kAct == MXB_ACT_GELU_TANH)
-    return z * logistic(2.0f * kSqrt2OverPi * (z + kGeluCubic * z * z * z));
   return z;
 }
 
@@ -128,7 +112,7 @@ __device__ __forceinline__ void logistic_pairs(const F2 (&z)[kP], F2 (&s)[kP]) {
   }
 }
 
-// normal_tail() of kP pairs, as the factor of gelu: 1 - q where z > 0, else q.
+// The factor of gelu for kP pairs: 1 - q(z) where z > 0, else q(z); and exp(-z^2 / 2).
 template <int kP>
 __device__ __forceinline__ void normal_cdf_pairs(const float* v, const F2 (&z)[kP], F2 (&cdf)[kP],
                                                  F2 (&gauss)[kP]) {
@@ -167,8 +151,8 @@ __device__ __forceinline__ F2 tanh_arg(F2 z) {
 
 // Eight values at a time, step by step and in pairs: a value alone is a chain of
 // dependent instructions (about 110 cycles for gelu), and the epilogue has two
-// warps a scheduler to hide it with.  The same arithmetic as act_value(), in
-// packed f32 instructions (gelu: 12 instead of 23 a value).
+// warps a scheduler to hide it with; in packed f32 instructions (gelu: 12 a value
+// instead of 23).
 template <int kAct>
 __device__ __forceinline__ void act8(float* v) {
   constexpr int kP = 4;

@@ -4,14 +4,14 @@
 // Rows are sorted by expert and the split is ragged and only known on the
 // device: every CTA builds the running sums of m_splits in shared memory and
 // walks tiles of (expert, row block, column block).  A's rows start anywhere, so
-// its E8M0 bytes are read row by row from the row-major layout that the
-// quantizer and the permute write, and put into the 128x4 atoms of the tcgen05
-// block-scale layout on the way to shared memory; a tile's rows past its
-// group's end are computed and not written.
+// its E8M0 bytes are read from the row-major layout that the quantizer and the
+// permute write, and put into the order of the tcgen05 block-scale layout on the
+// way to tensor memory; a tile's rows past its group's end are computed and not
+// written.
 //
 // Two kernels, chosen by grouped_plan() below:
-//   wide    256 rows x 256 weight rows a tile: the rows are the M side of MMAs
-//           that two CTAs share.
+//   wide    256 rows x 256 or 128 weight rows a tile: the rows are the M side of
+//           MMAs that two CTAs share.
 //   narrow  16 or 64 rows x 128 (gated: 256) weight rows a tile: the weights are
 //           the M side, so that a few rows do not pay for 128.  A cluster of up
 //           to 8 CTAs splits K; the partial accumulators meet in distributed

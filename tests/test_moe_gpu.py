@@ -112,6 +112,28 @@ def test_quantized_result_is_the_quantizer_on_c(cuda, E, M, W, K, name):
     assert torch.equal(q2, rq) and torch.equal(s2, rs)
 
 
+@pytest.mark.parametrize("M", [4, 3000])
+@pytest.mark.parametrize("name", R.ACTS)
+def test_activations_alone(cuda, M, name):
+    """Zero operands leave the bias: act(z) over z in [-80, 80], the tails included, against the
+    64-bit formula without cancellation.  One rounding to BF16 (2^-9, 2^-8 allowed) and the f32
+    evaluation (2^-16: an exponent of up to 115 rounded to f32); below 1e-36 f32 may underflow."""
+    W = 4096
+    gated = name == "swiglu"
+    z = torch.cat((torch.linspace(-80, 80, W // 2), torch.linspace(-6, 6, W // 2))).cuda()
+    bias = torch.cat((z, torch.linspace(-3, 3, W).cuda())) if gated else z
+    N = bias.numel()
+    ac = torch.zeros(M, 16, dtype=torch.uint8, device=cuda)
+    asc = torch.full((M, 1), 127, dtype=torch.uint8, device=cuda)
+    bc = torch.zeros(N, 16, dtype=torch.uint8, device=cuda)
+    bt = moe.omo_swizzle_scales_grouped(torch.full((1, N, 1), 127, dtype=torch.uint8, device=cuda), gated)
+    c = moe.omo_gemm_mxfp4_act(ac, asc, bc, bt[0], bias=bias, activation=name)
+    d = bias.double()
+    want = 0.5 * d * torch.special.erfc(-d / math.sqrt(2)) if name == "gelu" else \
+        d * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (d + 0.044715 * d ** 3)) if name == "gelu_tanh" else R.act(d, name)
+    R.check(c, want.expand(M, -1), (2.0 ** -8 + 2.0 ** -16) * want.abs().expand(M, -1) + 1e-36)
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 7168, 2048), (77, 1000, 1056), (129, 264, 4096), (300, 9600, 512)])
 @pytest.mark.parametrize("name", ["none", "silu", "swiglu"])
 def test_dense(cuda, M, N, K, name):
