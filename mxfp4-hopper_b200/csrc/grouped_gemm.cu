@@ -87,6 +87,17 @@ __device__ __forceinline__ bool scale_words(const GroupedArgs& p) {
            (uintptr_t)(p.K / 32)) & 3) == 0;
 }
 
+// 16 bytes from byte `at` (0 .. 15) of two neighbouring lines on.
+__device__ __forceinline__ uint4 bytes_from(const uint4& x, const uint4& y, uint32_t at) {
+  const bool two = at & 8, one = at & 4;
+  const uint32_t d0 = two ? x.z : x.x, d1 = two ? x.w : x.y, d2 = two ? y.x : x.z,
+                 d3 = two ? y.y : x.w, d4 = two ? y.z : y.x, d5 = two ? y.w : y.y;
+  const uint32_t e0 = one ? d1 : d0, e1 = one ? d2 : d1, e2 = one ? d3 : d2, e3 = one ? d4 : d3,
+                 e4 = one ? d5 : d4, sh = at % 4 * 8;
+  return make_uint4(__funnelshift_r(e0, e1, sh), __funnelshift_r(e1, e2, sh),
+                    __funnelshift_r(e2, e3, sh), __funnelshift_r(e3, e4, sh));
+}
+
 // 32 BF16 columns of a row: in 32-byte sectors where base and pitch allow it, else in
 // 16-byte pieces; columns past the `cols` there are (a multiple of 8) are left alone.
 __device__ __forceinline__ bool sectors(const void* base, int64_t ld) {
@@ -139,12 +150,18 @@ __device__ __forceinline__ float load_bias(const GroupedArgs& p, int64_t i) {
 //   warp 1       (CTA 0) MMA issue: four M = 256, N = kN, K = 64 a step
 //   warp 2       scales of four K steps at a time: a TMA box of 32 bytes of each
 //                of A's rows, bulk copies of B's atoms (both halves)
+//   warp 3       (kLines) A's scale rows that TMA cannot take, their base or pitch
+//                not being a multiple of 16: the three 16-byte lines that hold a
+//                row's 32 bytes, by cp.async, whose completion counts on warp 2's
+//                barrier.  Byte loads by the scale warps took 186 instead of 166 us
+//                (16384 rows over 32 experts, gated 2 x 2880 x 2880) and 51.5
+//                instead of 40.9 (4096 x 4096 x 4160); with both kinds of row in one
+//                kernel those of TMA became 4 % slower
 //   warps 4-7    scales: each warp gathers its lane quadrant's words of a step
 //                from shared memory and writes them to the step's tensor memory
 //                columns with tcgen05.st, so that the tensor pipe carries MMAs
 //                only, and arrives on the barrier that the codes complete on:
-//                one wait a step.  Rows that TMA cannot take (a pitch that is not
-//                a multiple of 16) are read by these warps, a row a thread
+//                one wait a step
 //   warps 8-15   epilogue: two groups of four warps, each with half the columns.
 //                The accumulator is read into registers at once and given back,
 //                so that the next tile's products run under the epilogue.  A
@@ -155,7 +172,8 @@ constexpr uint32_t kBoxBytes = 128 * 128;  // 128 rows of 128 code bytes
 constexpr uint32_t kAtoms = 2 * 512;       // scale atoms of 128 rows and one K step
 constexpr uint32_t kWideStage = 2 * kBoxBytes;
 constexpr int kSbStages = 2;               // shared-memory scales of four steps each:
-constexpr uint32_t kSbA = 128 * 32;        // A's 128 rows of 32 bytes,
+constexpr uint32_t kLineRow = 48;          // A's 128 rows of 32 bytes, or of three lines,
+constexpr uint32_t kSbA = 128 * kLineRow;
 constexpr uint32_t kSbB = 4 * kAtoms;      // 8 atoms of each of B's halves
 constexpr uint32_t kSbStage = kSbA + 2 * kSbB;
 constexpr uint32_t kScaleCol = 256;        // tensor memory: accumulator, then scales
@@ -169,7 +187,7 @@ static_assert(kWideStage % 1024 == 0, "swizzled boxes start on 1024 bytes");
 // scale warps must not spill: a spilled load is waited for where it is issued.
 constexpr int kWideCopyRegs = 64, kWideScaleRegs = 96, kWideEpilogueRegs = 176;
 
-template <int kAct, int kN>
+template <int kAct, int kN, bool kLines>
 __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
     const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
     const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ GroupedArgs p) {
@@ -211,7 +229,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < kSbStages; ++s) {
-      mbar_init(&sb_full[s], 1);
+      mbar_init(&sb_full[s], kLines ? 1 + 32 : 1);
       mbar_init(&sb_empty[s], 4);
     }
     mbar_init(acc_full, 1);
@@ -299,14 +317,52 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
           uint8_t* sb = scales + s * kSbStage;
           const uint32_t atoms = (uint32_t)min(8, S4 - k4) * 512;
           const bool two = kTwoBlocks && second;
-          mbar_arrive_expect_tx(&sb_full[s], (p.a_scales_tma ? kSbA : 0) + (two ? 2 : 1) * atoms);
-          if (p.a_scales_tma) tma_load_2d(sb, &map_sa, 4 * k4, tl.m0, &sb_full[s]);
+          mbar_arrive_expect_tx(&sb_full[s], (kLines ? 0 : 128 * 32) + (two ? 2 : 1) * atoms);
+          if (!kLines) tma_load_2d(sb, &map_sa, 4 * k4, tl.m0, &sb_full[s]);
           bulk_load_1d(sb + kSbA, src0 + k4 * 512, atoms, &sb_full[s]);
           if (two) bulk_load_1d(sb + kSbA + kSbB, src1 + k4 * 512, atoms, &sb_full[s]);
         }
       }
       for (int q = gq > kSbStages ? gq - kSbStages : 0; q < gq; ++q)
         mbar_wait_suspend(&sb_full[q % kSbStages], (uint32_t)((q / kSbStages) & 1));
+    } else if (kLines && warp == 3) {
+      // ------------------------------------------------ A's scale rows, four steps a time
+      int gq = 0;
+      bool ok = true;
+      for (int i = 0; ok && i < my_tiles; ++i) {
+        const Tile tl = tile_at(i);
+        const uint8_t* const row0 = p.a_scales + ((int64_t)tl.m0 + lane) * p.a_spitch;
+        const int rows = (int)min((int64_t)128, p.M - tl.m0);
+        for (int b0 = 0; b0 < S; b0 += 32, ++gq) {
+          const int s = gq % kSbStages;
+          const bool free = gq < kSbStages ||
+                            mbar_wait_suspend(&sb_empty[s], (uint32_t)((gq / kSbStages - 1) & 1));
+          if (!__all_sync(0xffffffffu, free)) {
+            atomicExch(failed, 1);
+            ok = false;
+            break;
+          }
+          const uint32_t sb = smem_addr(scales + s * kSbStage) + lane * kLineRow;
+          const uint8_t* from = row0 + b0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k, from += 32 * p.a_spitch) {
+            // the row's 32 bytes, or what is left of it; the rest becomes zero.  What the
+            // first line holds before them is read and not used (an allocation starts on
+            // a line, so a line with a byte of it lies in it).
+            const bool there = 32 * k + lane < rows;
+            const uint8_t* line = there ? from : p.a_scales;
+            const int before = (int)(reinterpret_cast<uintptr_t>(line) & 15u);
+            line -= before;
+            const int end = there ? before + min(32, S - b0) : 0;
+#pragma unroll
+            for (int c = 0; c < 3; ++c)
+              cp_async16_zfill(sb + k * 32 * kLineRow + 16 * c, line + (end > 16 * c ? 16 * c : 0),
+                               (uint32_t)max(0, min(16, end - 16 * c)));
+          }
+          cp_async_arrive(&sb_full[s]);
+        }
+      }
+      cp_async_wait_all();
     } else if (warp == 1 && rank == 0) {
       // ------------------------------------------------ MMA issuer
       const bool one = elect_one();
@@ -355,21 +411,22 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
     const int q = warp - 4;
     const uint32_t full0 = peer_addr(smem_addr(full), 0);
     const uint32_t col0 = tmem + ((uint32_t)(q * 32) << 16) + kScaleCol;
-    const bool words = scale_words(p);
     int gs = 0, gq = 0;
     bool ok = true;
     for (int i = 0; ok && i < my_tiles; ++i) {
       const Tile tl = tile_at(i);
-      const int64_t row0 = (int64_t)tl.m0 + 32 * q;
+      // where the 32 bytes of row 32 c + lane start
+      uint32_t at[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        at[c] = kLines ? (uint32_t)(32 * c + lane) * kLineRow +
+                             (((uint32_t)reinterpret_cast<uintptr_t>(p.a_scales) +
+                               (uint32_t)(tl.m0 + 32 * c + lane) * (uint32_t)p.a_spitch) & 15u)
+                       : (uint32_t)(32 * c + lane) * 32;
       for (int ks0 = 0; ok && ks0 < ksteps; ks0 += 4, ++gq) {
         const int sq = gq % kSbStages;
         uint8_t* sb = scales + sq * kSbStage;
         bool up = mbar_wait_suspend(&sb_full[sq], (uint32_t)((gq / kSbStages) & 1));
-        if (!p.a_scales_tma) {
-          gather_scales(sb + 1024 * q, p.a_scales + row0 * p.a_spitch, p.a_spitch,
-                        (int)max((int64_t)0, min((int64_t)32, p.M - row0)), ks0 * 8, S, words);
-          up = !named_sync_or(3, 128, !up);
-        }
 #pragma unroll
         for (int j = 0; j < 4; j += 2) {
           const int two = min(2, ksteps - ks0 - j);
@@ -377,9 +434,21 @@ __global__ void __launch_bounds__(kWideThreads, 1) grouped_wide_kernel(
           // a row's 16 bytes are two steps of two atoms; the four rows of a lane fill
           // the atoms' four columns
           uint4 ra[4];
+          if constexpr (!kLines) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            ra[c] = *reinterpret_cast<const uint4*>(sb + (32 * c + lane) * 32 + j * 8);
+            for (int c = 0; c < 4; ++c) ra[c] = *reinterpret_cast<const uint4*>(sb + at[c] + j * 8);
+          } else {
+            // two whole lines of each row, shifted down
+            uint4 x[4], y[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const uint4* const l = reinterpret_cast<const uint4*>(sb + (at[c] & ~15u)) + j / 2;
+              x[c] = l[0];
+              y[c] = l[1];
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) ra[c] = bytes_from(x[c], y[c], at[c] & 15u);
+          }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             if (h >= two) break;
@@ -991,33 +1060,37 @@ Plan grouped_plan(const GroupedArgs& p, bool glu) {
       std::max(estimate(r.ranks > 1 ? 85 : 70, cdiv(blocks(64) * cdiv(p.width, 128) * r.ranks, sms),
                         cdiv(ksteps, r.ranks), glu ? 56 : 35, 35),
                weights / 580000);
-  // rows of scales that TMA cannot take are gathered once per tile
+  // rows of scales that TMA cannot take cost a little more a step
   const int64_t wide128 = std::max(estimate(60, cdiv(blocks(256) * cdiv(cols, 128), pairs), ksteps,
-                                            p.a_scales_tma ? 21 : 50, 22),
+                                            p.a_scales_tma ? 21 : 26, 22),
                                    weights / 490000);
   const int64_t wide256 = std::max(estimate(85, cdiv(blocks(256) * cdiv(cols, 256), pairs), ksteps,
-                                            p.a_scales_tma ? 31 : 50, 47),
+                                            p.a_scales_tma ? 31 : 35, 47),
                                    weights / 490000);
   if (narrow <= std::min(wide128, wide256)) return r;
   const int n = wide128 < wide256 ? 128 : 256;
   return Plan{256, 1, most_tiles(p.M, p.E, 256, cdiv(cols, n)), n};
 }
 
-template <int kAct, int kN>
+template <int kAct, int kN, bool kLines>
 mxb_status launch_wide_n(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& ts,
-                       const GroupedArgs& p, const Plan& plan, cudaStream_t s) {
+                         const GroupedArgs& p, const Plan& plan, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
-  MXB_REQUIRE(grant_smem((const void*)grouped_wide_kernel<kAct, kN>, kWideSmem, done), MXB_ERR_CUDA,
+  const auto kernel = grouped_wide_kernel<kAct, kN, kLines>;
+  MXB_REQUIRE(grant_smem((const void*)kernel, kWideSmem, done), MXB_ERR_CUDA,
               "grouped_gemm_mxfp4: cannot reserve shared memory");
-  return launch_cluster("grouped_gemm_mxfp4", grouped_wide_kernel<kAct, kN>,
+  return launch_cluster("grouped_gemm_mxfp4", kernel,
                         (unsigned)std::min<int64_t>(plan.tiles, std::max(1, sm_count() / 2)), 2,
                         kWideThreads, kWideSmem, s, ta, tb, ts, p);
 }
 template <int kAct>
 mxb_status launch_wide(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& ts,
                        const GroupedArgs& p, const Plan& plan, cudaStream_t s) {
-  return plan.n == 128 ? launch_wide_n<kAct, 128>(ta, tb, ts, p, plan, s)
-                       : launch_wide_n<kAct, 256>(ta, tb, ts, p, plan, s);
+  if (p.a_scales_tma)
+    return plan.n == 128 ? launch_wide_n<kAct, 128, false>(ta, tb, ts, p, plan, s)
+                         : launch_wide_n<kAct, 256, false>(ta, tb, ts, p, plan, s);
+  return plan.n == 128 ? launch_wide_n<kAct, 128, true>(ta, tb, ts, p, plan, s)
+                       : launch_wide_n<kAct, 256, true>(ta, tb, ts, p, plan, s);
 }
 
 template <bool kGlu, int kT>

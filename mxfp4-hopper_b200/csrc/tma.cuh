@@ -153,6 +153,21 @@ __device__ __forceinline__ void bulk_load_1d(void* dst, const void* src, uint32_
       : "memory");
 }
 
+// 16 bytes global -> shared, both 16-byte aligned; of the source only the first `bytes`
+// are read, the rest is written as zero.
+__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+// This thread's cp.async copies so far count as one of the barrier's arrivals once they
+// have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
 // 2-D tiled TMA store of a shared-memory box to global memory (bulk group).
 // Elements outside the tensor are not written.  The writing threads must have
 // executed fence_proxy_async_smem() and synchronised before this is issued.
