@@ -4,6 +4,10 @@
     experts.quantize_weights()                    # once per weight update
     out = experts(x, topk_idx, topk_w)            # x BF16 [T, H], ids [T, k], weights [T, k]
 
+Under expert parallelism the layer holds a rank's own experts and takes what the dispatch
+delivers: ids local to the rank, -1 where a token's expert is on another rank.  Such an entry
+adds nothing to its token and its weight's gradient is 0.
+
 Forward: the tokens are quantized once and permuted as MXFP4 rows; the gate and up product
 applies SwiGLU in its epilogue and hands its result on as MXFP4; the down product's rows
 are weighted and summed back per token.  Backward: the rows that wait for it are the
@@ -26,14 +30,18 @@ from omo_python_api import mxfp4_moe as M
 
 def expert_order(topk_idx: torch.Tensor, num_experts: int):
     """Where the rows of tokens routed to topk_idx [T, k] go when sorted by expert, tokens in
-    order within an expert: (dst int32 [T, k], m_splits int32 [E])."""
+    order within an expert: (dst int32 [T, k], m_splits int32 [E]).  An id outside
+    [0, num_experts), as the dispatchers' -1 for an expert of another rank, has no row: its dst
+    is -1 and no expert counts it."""
     flat = topk_idx.reshape(-1).long()
-    order = torch.sort(flat, stable=True).indices
+    here = (flat >= 0) & (flat < num_experts)
+    key = torch.where(here, flat, num_experts)  # rows of nobody sort last
+    order = torch.sort(key, stable=True).indices
     dst = torch.empty_like(order, dtype=torch.int32)
     dst[order] = torch.arange(flat.numel(), dtype=torch.int32, device=flat.device)
-    splits = torch.zeros(num_experts, dtype=torch.int32, device=flat.device)
-    splits.scatter_add_(0, flat, torch.ones_like(flat, dtype=torch.int32))
-    return dst.reshape(topk_idx.shape), splits
+    splits = torch.zeros(num_experts + 1, dtype=torch.int32, device=flat.device)
+    splits.scatter_add_(0, key, torch.ones_like(key, dtype=torch.int32))
+    return torch.where(here, dst, -1).reshape(topk_idx.shape), splits[:num_experts]
 
 
 class QuantizedWeights:
