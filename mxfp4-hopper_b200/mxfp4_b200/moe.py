@@ -14,7 +14,8 @@ are weighted and summed back per token.  Backward: the rows that wait for it are
 MXFP4 ones (4.25 bits a value) and the BF16 rows before the activation; the input gradients
 are the same products with the transposed weights, the weight gradients come from BF16
 output gradients and the saved MXFP4 rows.  Nothing synchronises with the host: the rows per
-expert stay on the device and the buffers hold T * k rows.
+expert stay on the device and the buffers hold T * k rows.  A second derivative through the
+layer (a penalty on its gradients) raises.
 
 A weight with an FP32 `main_grad` attribute of its shape (Megatron's gradient buffer) gets
 its gradient added there; any other gets `.grad` in its own dtype.
@@ -61,6 +62,21 @@ class QuantizedWeights:
         self.scales_t = M.omo_swizzle_scales_grouped(scales_t)
 
 
+class _FirstOrder(torch.autograd.Function):
+    """Gradients as they are, with a graph that refuses to be differentiated.  `anchor` is what
+    makes the graph: the gradients may not need one themselves and yet depend on saved tensors
+    that do (a loss that is the plain sum of the outputs)."""
+
+    @staticmethod
+    def forward(ctx, anchor, *grads):
+        return grads
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("MXFP4Experts has no second derivative: the operators of its backward "
+                           "pass are not differentiable")
+
+
 class _Experts(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, topk_w, w1, w2, q1, q2, dst, splits):
@@ -76,6 +92,17 @@ class _Experts(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout):
+        with torch.no_grad():
+            grads = _Experts._grads(ctx, dout)
+        if torch.is_grad_enabled():  # create_graph: autograd does not see through the operators
+            there = [i for i, g in enumerate(grads) if g is not None]
+            anchor = torch.zeros((), device=dout.device, requires_grad=True)
+            for i, g in zip(there, _FirstOrder.apply(anchor, *(grads[i] for i in there))):
+                grads[i] = g
+        return (*grads, None, None, None, None)
+
+    @staticmethod
+    def _grads(ctx, dout):
         xc, xs, pre, hc, hs, y, dst, topk_w, splits, w1, w2 = ctx.saved_tensors
         dy, dtopk, dyc, dys = M.omo_moe_unpermute_grad(dout.contiguous(), y, dst, topk_w,
                                                        quantize=True)
@@ -87,7 +114,7 @@ class _Experts(torch.autograd.Function):
             dxp = M.omo_grouped_gemm_mxfp4(dzc, dzs, ctx.q1.codes_t, ctx.q1.scales_t, splits)
             dx = M.omo_moe_unpermute(dxp, dst)
         dw1 = _weight_grad(w1, dz, xc, xs, splits)
-        return dx, dtopk, dw1, dw2, None, None, None, None
+        return [dx, dtopk, dw1, dw2]
 
 
 def _weight_grad(w, dy, xc, xs, splits):

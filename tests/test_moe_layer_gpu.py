@@ -110,3 +110,19 @@ def test_layer_step_by_step(cuda, T, E, k, Hd, F, dtype, lost):
     R.check(x.grad, want, 2.0 ** -8 * want.abs() + k * 2.0 ** -23 * mag + 1e-40, "x's gradient")
     torch.cuda.synchronize()
     assert capi.reset_wait_timeouts() == 0
+
+
+def test_second_derivative_is_refused(cuda):
+    """With a graph of gradients the first ones are the same bytes, and a penalty on them raises."""
+    layer = MXFP4Experts(3, 128, 64, device=cuda)
+    layer.quantize_weights()
+    x = torch.randn(9, 128, device=cuda).to(BF).requires_grad_(True)
+    idx = torch.stack([torch.randperm(3, device=cuda)[:2] for _ in range(9)])
+    w = torch.rand(9, 2, device=cuda).requires_grad_(True)
+    inputs = (x, w, layer.w1, layer.w2)
+    want = torch.autograd.grad(layer(x, idx, w).sum(), inputs)
+    got = torch.autograd.grad(layer(x, idx, w).sum(), inputs, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for g in got:
+        with pytest.raises(RuntimeError, match="second derivative"):
+            g.float().square().sum().backward(retain_graph=True)
