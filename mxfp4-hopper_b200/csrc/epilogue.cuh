@@ -203,10 +203,17 @@ __device__ __forceinline__ void slope8(const float* v, float* out) {
       }
 #pragma unroll
       for (int i = 0; i < kP; ++i) {
-        F2 zs = mul2(z[i], s[i]);
-        if constexpr (kAct == MXB_ACT_GELU_TANH)
-          zs = mul2(zs, fma2(mul2(z[i], z[i]), both(6.0f * kSqrt2OverPi * kGeluCubic),
-                             both(2.0f * kSqrt2OverPi)));
+        F2 zs;
+        if constexpr (kAct == MXB_ACT_GELU_TANH) {
+          // z bounded: past +-32 s is exactly 0 or 1, and z^3 must not become an infinity
+          // that meets s (1 - s) = 0 (it does from 1.3e13 on)
+          const F2 c(fminf(fmaxf(v[2 * i], -32.0f), 32.0f),
+                     fminf(fmaxf(v[2 * i + 1], -32.0f), 32.0f));
+          zs = mul2(mul2(c, s[i]), fma2(mul2(c, c), both(6.0f * kSqrt2OverPi * kGeluCubic),
+                                        both(2.0f * kSqrt2OverPi)));
+        } else {
+          zs = mul2(z[i], s[i]);
+        }
         o[i] = fma2(zs, fma2(s[i], both(-1.0f), both(1.0f)), s[i]);
       }
     }
