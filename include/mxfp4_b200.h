@@ -334,6 +334,14 @@ mxb_status mxb_grouped_gemm_mxfp4(const void* a_codes, int64_t a_codes_pitch, co
                                   int64_t K, const mxb_epilogue* epilogue, void* c,
                                   mxb_stream_t stream);
 
+/* How such a call is done on the current device, for tests and measurements (host only, nothing
+ * is launched): plan[0] rows of a tile (256: the wide kernel; 64, 16: the narrow one), [1] weight
+ * rows of a tile, [2] CTAs that split K, [3] the most tiles that any split has, [4] clusters
+ * that share them.  quantized: c_codes is given; scale_rows_aligned: a_scales and its
+ * pitch are multiples of 16. */
+mxb_status mxb_grouped_gemm_plan(int64_t M, int32_t E, int64_t N, int64_t K, int32_t activation,
+                                 int32_t quantized, int32_t scale_rows_aligned, int64_t plan[5]);
+
 /* The experts' weight gradients: dw[e] [N, K] = sum over the rows r of expert e
  * of dy[r]^T x[r], with dy bf16 [M, N] (pitch dy_ld elements, a multiple of 8)
  * and x the saved MXFP4 rows (codes [M, K/2] and E8M0 scales [M, K/32], pitches

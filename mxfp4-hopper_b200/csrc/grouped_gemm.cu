@@ -1072,6 +1072,11 @@ Plan grouped_plan(const GroupedArgs& p, bool glu) {
   return Plan{256, 1, most_tiles(p.M, p.E, 256, cdiv(cols, n)), n};
 }
 
+// Persistent clusters, which share the tiles: pairs of CTAs (wide), or those that split K.
+int64_t clusters_of(const Plan& plan) {
+  return std::min<int64_t>(plan.tiles, std::max(1, sm_count() / (plan.n ? 2 : plan.ranks)));
+}
+
 template <int kAct, int kN, bool kLines>
 mxb_status launch_wide_n(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& ts,
                          const GroupedArgs& p, const Plan& plan, cudaStream_t s) {
@@ -1080,8 +1085,7 @@ mxb_status launch_wide_n(const CUtensorMap& ta, const CUtensorMap& tb, const CUt
   MXB_REQUIRE(grant_smem((const void*)kernel, kWideSmem, done), MXB_ERR_CUDA,
               "grouped_gemm_mxfp4: cannot reserve shared memory");
   return launch_cluster("grouped_gemm_mxfp4", kernel,
-                        (unsigned)std::min<int64_t>(plan.tiles, std::max(1, sm_count() / 2)), 2,
-                        kWideThreads, kWideSmem, s, ta, tb, ts, p);
+                        (unsigned)clusters_of(plan), 2, kWideThreads, kWideSmem, s, ta, tb, ts, p);
 }
 template <int kAct>
 mxb_status launch_wide(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& ts,
@@ -1100,9 +1104,9 @@ mxb_status launch_narrow(const CUtensorMap& ta, const CUtensorMap& tb, const Gro
   static std::atomic<uint64_t> done{0};
   MXB_REQUIRE(grant_smem((const void*)grouped_narrow_kernel<kGlu, kT>, L::kSmem, done),
               MXB_ERR_CUDA, "grouped_gemm_mxfp4: cannot reserve shared memory");
-  const int64_t clusters = std::min<int64_t>(plan.tiles, std::max(1, sm_count() / plan.ranks));
-  return launch_cluster("grouped_gemm_mxfp4", grouped_narrow_kernel<kGlu, kT>, (unsigned)clusters, (unsigned)plan.ranks,
-                        kNarrowThreads, L::kSmem, s, ta, tb, p);
+  return launch_cluster("grouped_gemm_mxfp4", grouped_narrow_kernel<kGlu, kT>,
+                        (unsigned)clusters_of(plan), (unsigned)plan.ranks, kNarrowThreads, L::kSmem,
+                        s, ta, tb, p);
 }
 
 }  // namespace
@@ -1127,6 +1131,31 @@ extern "C" mxb_status mxb_swizzle_scales_grouped(const void* scales, int64_t E, 
                            to_cuda(stream)>>>((const uint8_t*)scales, E * parts, N / parts, (int)S,
                                               (uint32_t*)out);
   return launch_status("swizzle_scales_grouped");
+}
+
+extern "C" mxb_status mxb_grouped_gemm_plan(int64_t M, int32_t E, int64_t N, int64_t K,
+                                            int32_t activation, int32_t quantized,
+                                            int32_t scale_rows_aligned, int64_t plan[5]) {
+  const bool glu = activation == MXB_ACT_SWIGLU;
+  MXB_REQUIRE(plan && M >= 1 && M <= INT32_MAX - 512 && E >= 1 && E <= MXB_MAX_EXPERTS && N >= 1 &&
+                  N % (glu ? 16 : 8) == 0 && (int64_t)E * N <= INT32_MAX - 512 && K >= 32 &&
+                  K % 32 == 0 && K <= (1 << 24) && activation >= MXB_ACT_NONE &&
+                  activation <= MXB_ACT_SWIGLU,
+              MXB_ERR_INVALID_ARGUMENT,
+              "grouped_gemm_plan: need a plan and a call's sizes (M=%lld E=%d N=%lld K=%lld)",
+              (long long)M, E, (long long)N, (long long)K);
+  GroupedArgs p = {};
+  p.M = M;
+  p.E = E;
+  p.width = (int)(N / (glu ? 2 : 1));
+  p.K = (int)K;
+  uint8_t some = 0;
+  p.c_codes = quantized ? &some : nullptr;
+  p.a_scales_tma = scale_rows_aligned != 0;
+  const Plan r = grouped_plan(p, glu);
+  const int64_t values[5] = {r.rows, r.n ? r.n : glu ? 256 : 128, r.ranks, r.tiles, clusters_of(r)};
+  std::copy(values, values + 5, plan);
+  return MXB_OK;
 }
 
 extern "C" mxb_status mxb_grouped_gemm_mxfp4(const void* a_codes, int64_t a_codes_pitch,

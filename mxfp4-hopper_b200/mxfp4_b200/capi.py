@@ -114,6 +114,7 @@ _EP = ctypes.POINTER(Epilogue)
 SIGNATURES.update({
     "mxb_swizzle_scales_grouped": [_P, _I64, _I64, _I64, _I32, _P, _P],
     "mxb_grouped_gemm_mxfp4": [_P, _I64, _P, _I64, _I64, _P, _I32, _P, _P, _I64, _I64, _EP, _P, _P],
+    "mxb_grouped_gemm_plan": [_I64, _I32, _I64, _I64, _I32, _I32, _I32, _P],
     "mxb_grouped_wgrad_mxfp4": [_P, _I64, _P, _I64, _P, _I64, _I64, _P, _I32, _I64, _I64, _P, _I32,
                                 _I32, _P],
     "mxb_bias_act_grad": [_P, _P, _I64, _P, _I32, _I64, _I32, _P, _P, _P, _P, _P, _I64, _P],
