@@ -10,11 +10,14 @@
 //              written with the logistic function, (1 + tanh u) / 2 = s(2 u)
 //   swiglu     silu(gate) * up, gate and up from two halves of the columns
 //
-// The logistic function uses the hardware exponential and reciprocal (about
-// 2^-22 relative), which a BF16 result cannot tell from exact.  q(z) is taken as
-// t P(t) exp(-z^2 / 2) with t = 1 / (1 + 0.3 |z|) and P a polynomial of degree 7
-// fitted here to erfc in relative error (least squares on Chebyshev nodes of t,
-// reweighted towards the minimax; 1.5e-7 for |z| <= 14, past which q underflows).
+// The logistic function uses the hardware exponential and reciprocal: about 2^-22
+// relative, and |z| 2^-23 more for the rounded exponent, which a BF16 result cannot tell
+// from exact.  Below 2^-126 it is 0: silu is -0 for z < -87.3, where it should be
+// at most 1.03e-36 in size.  q(z) is taken as t P(t) exp(-z^2 / 2) with t = 1 / (1 + 0.3 |z|)
+// and P a polynomial of degree 7 fitted here to erfc in relative error (least squares on
+// Chebyshev nodes of t, reweighted towards the minimax: 1.7e-7 for |z| <= 14 with the
+// coefficients in f32; the exponent's rounding adds z^2 2^-24).  From |z| = 13.2 on
+// the exponential is 0, and with it z q, which is below 2^-126 there.
 // With erff, whose two ranges a warp both runs, the epilogue of an 8192^2 x 7168
 // product took 14.7 thousand cycles a tile for the activation alone, longer than the
 // tile's products.

@@ -183,8 +183,10 @@ constexpr size_t kWideSmem = 1024 + kWideStages * kWideStage + kSbStages * kSbSt
 static_assert(kWideSmem <= 227 * 1024, "one CTA per SM");
 static_assert(kScaleCol + 24 * kWideStages <= kTmemCols, "scales fit beside the accumulator");
 static_assert(kWideStage % 1024 == 0, "swizzled boxes start on 1024 bytes");
-// Registers: 512 threads x 128 at launch = 128 x 64 + 128 x 96 + 256 x 176.  The
-// scale warps must not spill: a spilled load is waited for where it is issued.
+// Registers: 512 threads x 128 at launch = 128 x 64 + 128 x 96 + 256 x 176.  (A scale
+// warp should not spill: a spilled load is waited for where it is issued.  The compiler
+// reports 64 spilled bytes for the kernels of 256 weight rows, 20 where gated, and up to
+// 4 (stored; 32 reloaded) for those of 128, 20 (140) where gated with TMA's scale rows.)
 constexpr int kWideCopyRegs = 64, kWideScaleRegs = 96, kWideEpilogueRegs = 176;
 
 template <int kAct, int kN, bool kLines>
@@ -1026,9 +1028,11 @@ int64_t most_tiles(int64_t M, int64_t E, int rows, int64_t ntn) {
 // Few rows an expert (the weights' bytes are the time): narrow.  Else the least of three
 // estimates in tenths of a microsecond, each a start with the last tile's epilogue, so
 // much a K step, and a further round of tiles at the longer of its steps and an
-// epilogue; at least the weights' bytes at the rate each reaches.  The coefficients were
-// read off products of 40 to 8192 rows, e.g. (us, narrow / 128 / 256 weight rows a
-// tile): 200 x 1024 x 256 7.9 / 6.3 / 8.5; 300 x 3600 x 4096 13.3 / 9.6 / 13.1;
+// epilogue; at least the weights' bytes at the rate each reaches.  They order the variants
+// and are no prediction: epilogue operands and rows that start inside a sector are not in
+// them (3001 rows over 16 experts of 1416 x 2080 with bias and gelu_tanh: 16.3 against 24.2
+// us measured).  The coefficients were read off products without epilogue operands of 40 to
+// 8192 rows, e.g. (us, narrow / 128 / 256 weight rows a tile): 200 x 1024 x 256 7.9 / 6.3 / 8.5; 300 x 3600 x 4096 13.3 / 9.6 / 13.1;
 // 130 x 512 x 7168, where narrow splits K eight ways, 8.8 / 11.2 / 16.0;
 // 1500 x 2048 x 2048 19.4 / 10.5 / 12.0; 2000 x 4096 x 4096 43.9 / 23.9 / 21.5;
 // 1500 rows over 32 experts of 4096 x 7168 96 / 132 / 103.

@@ -11,7 +11,9 @@ adds nothing to its token and its weight's gradient is 0.
 Forward: the tokens are quantized once and permuted as MXFP4 rows; the gate and up product
 applies SwiGLU in its epilogue and hands its result on as MXFP4; the down product's rows
 are weighted and summed back per token.  Backward: the rows that wait for it are the
-MXFP4 ones (4.25 bits a value) and the BF16 rows before the activation; the input gradients
+MXFP4 ones of both products (4.25 bits a value) and, in BF16, the rows before the activation
+[T * k, 2F] and the down product's [T * k, H], which the routing weights' gradient needs; they
+are made and kept whether or not a gradient is asked for.  The input gradients
 are the same products with the transposed weights, the weight gradients come from BF16
 output gradients and the saved MXFP4 rows.  Nothing synchronises with the host: the rows per
 expert stay on the device and the buffers hold T * k rows.  A second derivative through the
